@@ -4,6 +4,7 @@ import ctypes as C
 FMT_REF_NVFP4, FMT_REF_INT4, FMT_REF_BF16 = 0, 2, 3
 FMT_FP8, FMT_INT4, FMT_BF16 = 16, 18, 19
 FMT_MXFP4, FMT_FP8E = 20, 21  # DeepSeek's routed experts; their shared expert (ue8m0 scales per 32 x 32)
+KV_E4M3 = 22  # a cache of e4m3 codes with a scale a head
 OUT_BF16, OUT_F32, OUT_SWIGLU = 0, 1, 2
 MAX_ROWS, MAX_TOPK, MAX_UNION, SH_SLOT, MAX_EXPERTS, MAX_CHUNK = 16, 8, 128, 128, 512, 8192
 UP_PREFILL_ORDER = 6  # dsgx_decode_cfg.up: the rows through the prefill kernels (gx::kUpPrefillOrder), bf16 activations
@@ -66,6 +67,26 @@ class GemvSeg(C.Structure):
                 ("rs", C.c_int32), ("ks", C.c_int32), ("y", C.c_void_p), ("ldy", C.c_int32)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ks", "vs")] + [(n, C.c_int64) for n in ("page_stride", "tok_stride", "head_stride")] + \
+               [("fmt", C.c_uint32)] + [(n, C.c_int32) for n in ("Hkv", "D", "page", "npages")]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("cu_rows", "lens", "table", "prefix")] + \
+               [(n, C.c_int32) for n in ("B", "rows", "max_rows", "max_len", "table_ld", "prefix_len")]
+
+
+class KvAppendIn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "q_norm", "k_norm", "rope", "pos")] + [(n, C.c_int64) for n in ("ldq", "ldk", "ldv", "ldqo")] + \
+               [(n, C.c_int32) for n in ("Hq", "rot", "rot_off", "pairs", "rope_len")] + [("eps", C.c_float)]
+
+
+class VerifyIn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("target", "q", "draft", "cu_rows", "u", "us", "temp")] + [(n, C.c_int64) for n in ("ldt", "ldq")] + \
+               [(n, C.c_int32) for n in ("kind", "V", "B", "rows", "max_rows")]
+
+
 assert C.sizeof(MatDesc) == 64
 
 # every symbol include/dsgx.h declares
@@ -75,4 +96,5 @@ SYMBOLS = [
     "dsgx_moe_prefill", "dsgx_prefill_view_get", "dsgx_gemv", "dsgx_dequant_int4", "dsgx_probe_dequant_int4", "dsgx_probe_dequant_int4_any", "dsgx_probe_mfma_fp8",
     "dsgx_widen_fp8", "dsgx_act_quant", "dsgx_last_error", "dsgx_version", "dsgx_stream_read", "dsgx_stream_read_cfg", "dsgx_stream_copy", "dsgx_add_norm_gemv", "dsgx_fill_normal", "dsgx_launch_floor",
     "dsgx_dsk_prefill_cfg_default", "dsgx_dsk_prefill_ws_bytes", "dsgx_dsk_moe_prefill", "dsgx_dsk_prefill_view_get", "dsgx_probe_mfma_scaled", "dsgx_probe_mfma_bf16", "dsgx_probe_dot2_bf16",
+    "dsgx_kv_append", "dsgx_attn_ws_bytes", "dsgx_attn", "dsgx_spec_verify_ws_bytes", "dsgx_spec_verify",
 ]

@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(CSRC, "libdsgx.so")
 SOURCES = ["abi.hip", "route.hip", "gemv.hip", "moe_decode.hip", "moe_decode_fp8.hip", "moe_decode_int4.hip", "moe_decode_int4_mfma.hip", "moe_decode_mxfp4_mfma.hip",
-           "moe_decode_bf16.hip", "moe_prefill.hip"]
+           "moe_decode_bf16.hip", "moe_prefill.hip", "kv_append.hip", "attn.hip", "spec_verify.hip"]
 # -packed-fp32-ops off: hipcc -O3 otherwise forms v_pk_*_f32 from scalar float code
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]

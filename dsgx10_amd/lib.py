@@ -73,6 +73,14 @@ def lib():
         L.dsgx_add_norm_gemv.argtypes = [C.POINTER(abi.NormIn), C.c_int, C.c_int, C.POINTER(abi.GemvSeg), C.c_int, C.c_int, C.c_int, C.c_void_p]
         L.dsgx_fill_normal.argtypes = [C.c_uint64, C.c_uint64, C.c_size_t, C.c_double, C.c_void_p, C.c_int, C.c_void_p]
         L.dsgx_launch_floor.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
+        L.dsgx_kv_append.argtypes = [C.POINTER(abi.KvCache), C.POINTER(abi.KvBatch), C.POINTER(abi.KvAppendIn), C.c_void_p]
+        L.dsgx_attn_ws_bytes.restype = C.c_size_t
+        L.dsgx_attn_ws_bytes.argtypes = [C.POINTER(abi.KvCache), C.POINTER(abi.KvBatch), C.c_int]
+        L.dsgx_attn.argtypes = [C.POINTER(abi.KvCache), C.POINTER(abi.KvBatch), C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_void_p, C.c_int64, C.c_void_p,
+                                C.c_void_p, C.c_void_p]
+        L.dsgx_spec_verify_ws_bytes.restype = C.c_size_t
+        L.dsgx_spec_verify_ws_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+        L.dsgx_spec_verify.argtypes = [C.POINTER(abi.VerifyIn), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
         if hasattr(L, "dsgx_moe_prefill"):
             L.dsgx_prefill_ws_bytes.restype = C.c_size_t
             L.dsgx_prefill_ws_bytes.argtypes = [C.POINTER(abi.LayerW), C.c_int]
@@ -273,3 +281,58 @@ def probe_mfma_fp8(A, B, raw, form=0, stream=None):
     """raw f32 [64][16]: the accumulator registers of one e4m3 MFMA; form 0: 32x32x64 over A [32][64], B [32][64];
     form 1: 16x16x128 over A [16][128], B [16][128]"""
     _check(lib().dsgx_probe_mfma_fp8(_ptr(A), _ptr(B), _ptr(raw), form, _stream(stream)))
+
+
+# ---- the attention side of a decode step ------------------------------------------------------------------------------------
+def kv_cache(k, v, ks=None, vs=None):
+    """The handle of a paged cache over two pools [npages][page][Hkv][D] (views of any strides whose last is 1): bf16, or e4m3 codes
+    (uint8 or float8_e4m3fn) with f32 scales ks, vs [Hkv]. It holds addresses: the pools have to live as long."""
+    n, page, Hkv, D = k.shape
+    if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or k.stride(3) != 1:
+        raise DsgxError(abi.EINVAL, "kv_cache: keys %s, values %s: two pools of the same shape, strides and type are needed" % (tuple(k.shape), tuple(v.shape)))
+    kind = {"torch.bfloat16": abi.FMT_BF16, "torch.uint16": abi.FMT_BF16, "torch.uint8": abi.KV_E4M3, "torch.float8_e4m3fn": abi.KV_E4M3}.get(str(k.dtype))
+    if kind is None or (kind == abi.KV_E4M3) != (ks is not None) or (ks is None) != (vs is None):
+        raise DsgxError(abi.EINVAL, "kv_cache: %s with scales %s, %s (bf16 without, e4m3 with)" % (k.dtype, None if ks is None else ks.dtype, None if vs is None else vs.dtype))
+    if ks is not None and any(str(t.dtype) != "torch.float32" or t.numel() != Hkv or not t.is_contiguous() for t in (ks, vs)):
+        raise DsgxError(abi.EINVAL, "kv_cache: the scales are contiguous f32 [%d]" % Hkv)
+    return abi.KvCache(_ptr(k), _ptr(v), _ptr(ks), _ptr(vs), k.stride(0), k.stride(1), k.stride(2), kind, Hkv, D, page, n)
+
+
+def kv_batch(rows, max_rows, max_len, lens, table, cu_rows=None, prefix_len=0, prefix=None):
+    """The handle of a step's sequences: lens i32 [B], table i32 [B][pages], cu_rows i32 [B + 1] or None (max_rows rows each), prefix i32
+    [ceil(prefix_len / page)]. It holds addresses: the kernels read the tensors' contents when they run."""
+    for t in (lens, table, cu_rows, prefix):
+        if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous()):
+            raise DsgxError(abi.EINVAL, "kv_batch: lens, table, cu_rows and prefix are contiguous 32-bit integers")
+    return abi.KvBatch(_ptr(cu_rows), _ptr(lens), _ptr(table), _ptr(prefix), table.shape[0], rows, max_rows, max_len, table.shape[1], prefix_len)
+
+
+def kv_append(cache, batch, k, ldk, v, ldv, q=None, ldq=0, Hq=0, q_out=None, ldqo=0, q_norm=None, k_norm=None, eps=1e-5, rope=None, rot=0, rot_off=0, pairs=False,
+              pos=None, stream=None):
+    """The step's rows on their way to attention: q and k normed per head and rotated, q to q_out, k and v into the cache"""
+    a = abi.KvAppendIn(_ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(q_norm), _ptr(k_norm), _ptr(rope), _ptr(pos), ldq, ldk, ldv, ldqo, Hq, rot, rot_off, int(pairs),
+                       0 if rope is None else rope.numel() // max(rot, 1), eps)
+    _check(lib().dsgx_kv_append(C.byref(cache), C.byref(batch), C.byref(a), _stream(stream)))
+
+
+def attn_ws_bytes(cache, batch, Hq):
+    return lib().dsgx_attn_ws_bytes(C.byref(cache), C.byref(batch), Hq)
+
+
+def attn(cache, batch, q, ldq, Hq, scale, out, ldo, ws, lse=None, stream=None):
+    """out = softmax(scale q K^T) V of the step's rows over the shared prefix and their sequences' own tokens; lse f32 [rows][Hq] optional"""
+    _check(lib().dsgx_attn(C.byref(cache), C.byref(batch), _ptr(q), ldq, Hq, scale, _ptr(out), ldo, _ptr(lse), _ptr(ws), _stream(stream)))
+
+
+def spec_verify_ws_bytes(B, rows, V):
+    return lib().dsgx_spec_verify_ws_bytes(B, rows, V)
+
+
+def spec_verify(target, V, draft, u, us, tokens, accepted, ws, max_rows, cu_rows=None, q=None, temp=None, probs=False, ldt=None, ldq=None, stream=None):
+    """Drafted tokens against the target (f32 or bf16 logits, or with probs f32 probabilities; rows V or ldt values apart): tokens i32 [rows], accepted i32 [B]"""
+    kind = {"torch.float32": 2 if probs else 0, "torch.bfloat16": None if probs else 1}.get(str(target.dtype))
+    if kind is None or (q is not None and str(q.dtype) != "torch.float32"):
+        raise DsgxError(abi.EINVAL, "spec_verify: a target of %s, a drafter's probabilities of %s" % (target.dtype, None if q is None else q.dtype))
+    a = abi.VerifyIn(_ptr(target), _ptr(q), _ptr(draft), _ptr(cu_rows), _ptr(u), _ptr(us), _ptr(temp), ldt or V, ldq or V, kind, V,
+                     accepted.numel(), tokens.numel(), max_rows)
+    _check(lib().dsgx_spec_verify(C.byref(a), _ptr(tokens), _ptr(accepted), _ptr(ws), _stream(stream)))

@@ -316,6 +316,96 @@ typedef struct dsgx_norm_in {
 DSGX_API int dsgx_add_norm_gemv(const dsgx_norm_in* n, int rows, int K, const dsgx_gemv_seg* segs, int nseg, int out, int splitk,
                                 void* stream);
 
+/* ---- the attention side of a decode step -------------------------------------------------------------------------------
+   What stands between the projections of a decode layer and after its head: the step's queries and keys normed, rotated and
+   appended to a paged cache of keys and values, attention over that cache for sequences that may share a prefix, and the
+   verification of drafted tokens. The reference's attention reads a compressed latent through an indexer
+   (altar1-4xgx10-switchless/engine/attn/attn.h:160-258, not part of this build); these operators keep whole heads.
+
+   A cache is two pools (keys and values) of pages of `page` tokens (a power of two, 16 .. 1024). A value lies at
+     page * page_stride + (token in the page) * tok_stride + kv head * head_stride + d        (strides in values, both pools alike)
+   so both orders of tokens and heads, and pools interleaved in one tensor, are caches; the D values of a head are contiguous.
+   fmt: DSGX_FMT_BF16, or DSGX_KV_E4M3 (e4m3fn codes; kv head h stands for code * ks[h], code * vs[h]; ks, vs f32 [Hkv] in device
+   memory, positive). D 64, 128 or 256. Pools and strides 16-byte aligned (in bytes). */
+enum { DSGX_KV_E4M3 = 22 };
+typedef struct dsgx_kv_cache {
+  void *k, *v;
+  const float *ks, *vs;
+  int64_t page_stride, tok_stride, head_stride;
+  uint32_t fmt;
+  int32_t Hkv, D, page, npages;
+} dsgx_kv_cache;
+
+/* The sequences of one step. Sequence b has the step's rows cu_rows[b] .. cu_rows[b + 1] - 1 and lens[b] tokens of its own, the
+   step's rows the last of them: its row i of n is its own token lens[b] - n + i. Own token t lies in page table[b][t / page].
+   In front of every sequence's own tokens stand prefix_len tokens that all share, token t in page prefix[t / page]; a
+   sequence's own tokens begin a page of their own, wherever the prefix ends.
+   Everything but the sizes is device memory, read when the kernels run, so a captured step replays with other lengths:
+   max_rows and max_len plan the launches (rows a sequence, own tokens a sequence); a sequence that passes them is still computed
+   right, only slower. cu_rows null: max_rows rows a sequence (rows = B * max_rows).
+   What the device arrays hold is not trusted: rows that no sequence has are left as they are; lens is cut to what `table_ld`
+   pages hold; a page number outside 0 .. npages - 1 is never followed (append: the token is not stored; attention: its
+   tokens are not there). */
+typedef struct dsgx_kv_batch {
+  const int32_t *cu_rows; /* [B + 1] or null */
+  const int32_t *lens;    /* [B] */
+  const int32_t *table;   /* [B][table_ld] */
+  const int32_t *prefix;  /* [ceil(prefix_len / page)]; null with prefix_len 0 */
+  int32_t B, rows, max_rows, max_len, table_ld, prefix_len;
+} dsgx_kv_batch;
+
+/* The step's rows on their way to attention, one pass: per head of q (Hq heads) and k (Hkv heads), f32 throughout,
+     y = x * rsqrt(mean(x^2) + eps) * norm           (norm bf16 [D], shared by the heads; null: y = x)
+     dims rot_off .. rot_off + rot - 1 of y rotated by the row's position: (a c - b s, b c + a s) with c = rope[pos][j],
+     s = rope[pos][rot / 2 + j] for the pair (a, b) = dims (j, j + rot / 2), or with `pairs` dims (2j, 2j + 1), after rot_off
+   then rounded once: q to bf16 in q_out (may be q itself), k and v (neither normed nor rotated) into the cache at the row's token,
+   to bf16 or to e4m3 of the value / the head's scale (nearest even, clamped to +-448; a NaN stays one).
+   pos: i32 [rows], or null: prefix_len + the row's own token. rope f32 [rope_len][rot] or null with rot 0. A position outside the
+   table: the row's q is NaN where it is rotated, its k and v are not stored. q null: keys and values alone.
+   Rows of q, k, v, q_out are ld* values apart, a row's heads D; all 16-byte aligned; rot, rot_off multiples of 16. */
+typedef struct dsgx_kv_append_in {
+  const uint16_t *q, *k, *v;
+  uint16_t* q_out;
+  const uint16_t *q_norm, *k_norm;
+  const float* rope;
+  const int32_t* pos;
+  int64_t ldq, ldk, ldv, ldqo;
+  int32_t Hq, rot, rot_off, pairs, rope_len;
+  float eps;
+} dsgx_kv_append_in;
+DSGX_API int dsgx_kv_append(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const dsgx_kv_append_in* in, void* stream);
+
+/* Attention of the step's rows over the cache: head a of row r attends with kv head a / (Hq / Hkv) to the prefix and to its
+   sequence's own tokens up to and with the row's own:
+     s = scale * q . k;  out = sum softmax(s) v rounded once to bf16;  lse (optional, f32 [rows][Hq]) = ln sum exp(s)
+   A row that sees nothing has out 0 and lse -inf. What a masked or unwritten place holds (NaN, infinities) does not reach a result.
+   Scores, softmax statistics and sums are f32; the softmax's numerators are rounded to bf16 for the matrix unit. q, out bf16
+   [rows][ld*], a row's Hq heads of D side by side, 16-byte aligned. The prefix is read once for all rows. ws:
+   dsgx_attn_ws_bytes(...) bytes of device memory, zeroed once; it belongs to one call at a time (calls in stream order share it). */
+DSGX_API size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, int Hq);
+DSGX_API int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale,
+                       uint16_t* out, int64_t ldo, float* lse, void* ws, void* stream);
+
+/* Verification of drafted tokens by rejection sampling from given random numbers, all in f64. Sequence b has the rows
+   cu_rows[b] .. cu_rows[b + 1] - 1 of the target (null: max_rows rows each), one more than it has drafts: row i judges draft i, the last
+   row follows them all. Row r: the target p_r = softmax(target[r] / temp[b]) (temp <= 0: all on the largest logit, the lowest id of
+   equals), or with probs target[r] itself; draft[r], u[r] in [0, 1) and the drafter's probabilities q[r] (null: the
+   drafter was sure of its token) are read for all rows but a sequence's last. Draft i is accepted while u q(draft) < p(draft); at the
+   first that is not, the next token is drawn from max(p - q, 0) (all zero: from p), after the last from p: the lowest id v with
+   sum(w[0 .. v]) > us[b] * sum(w). tokens [rows]: the accepted drafts, the drawn token, then -1; accepted [B].
+   A draft outside 0 .. V - 1 is refused; a row whose weights have no finite positive sum draws -1 (its draft is refused).
+   kind 0: f32 logits, 1: bf16 logits, 2: f32 probabilities. temp null: 1. ws: dsgx_spec_verify_ws_bytes(...) bytes, zeroed once. */
+typedef struct dsgx_verify_in {
+  const void* target;
+  const float* q;
+  const int32_t *draft, *cu_rows;
+  const float *u, *us, *temp;
+  int64_t ldt, ldq;
+  int32_t kind, V, B, rows, max_rows;
+} dsgx_verify_in;
+DSGX_API size_t dsgx_spec_verify_ws_bytes(int B, int rows, int V);
+DSGX_API int dsgx_spec_verify(const dsgx_verify_in* in, int32_t* tokens, int32_t* accepted, void* ws, void* stream);
+
 /* glm::dequant_int4 (engine/attn/attn.h:154-158): the contract's bf16 weight [N][ld] from the canonical tensors */
 DSGX_API int dsgx_dequant_int4(const void* packed, const void* scale, const void* zp, int N, int K, uint16_t* out,
                                size_t ld, void* stream);
