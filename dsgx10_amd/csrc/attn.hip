@@ -5,6 +5,8 @@
 // sequence's rows over its own tokens, all rows over the prefix. The tokens are cut into ranges, a workgroup each; what the ranges
 // leave (maximum, sum, unnormalised output in f32) k_combine joins.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -31,8 +33,45 @@ struct AttnArgs {
   float2* ml;
   int64_t ldq, ldo;
   int Hq, G, page_shift;
-  float scale2;  // scale * log2 e
+  float scale2;              // |scale| log2 e; 1 for a scale of zero
+  uint32_t q_flip, q_keep;   // the scale's sign and whether it is zero, on the queries' bits
 };
+
+// The tokens and rows of a workgroup: a range of the prefix for all rows, or of a sequence's own tokens for its rows
+struct Range {
+  const int32_t* tab;
+  int head, split, first, rows, len, lo, hi;  // lo .. hi - 1 of len tokens
+  bool any;
+};
+__device__ __forceinline__ Range range_of(const AttnArgs& a, int prefix) {
+  Range r{a.b.prefix, (int)blockIdx.x % a.c.Hkv, (int)blockIdx.x / a.c.Hkv, 0, a.b.rows, a.b.prefix_len, 0, 0, true};
+  if (!prefix) {
+    const int b = blockIdx.z;
+    r.first = a.b.cu_rows ? a.b.cu_rows[b] : b * a.b.max_rows;
+    const int end = a.b.cu_rows ? a.b.cu_rows[b + 1] : r.first + a.b.max_rows;
+    if (r.first < 0 || end <= r.first || end > a.b.rows) {
+      r.any = false;
+      return r;
+    }
+    r.rows = end - r.first;
+    const int cap = a.b.table_ld << a.page_shift, len = a.b.lens[b];
+    r.len = len < 0 ? 0 : len > cap ? cap : len;
+    r.tab = a.b.table + (size_t)b * a.b.table_ld;
+  }
+  const int chunk = prefix ? a.p.cp : a.p.co, splits = prefix ? a.p.sp : a.p.so;
+  r.lo = r.split * chunk, r.hi = r.split == splits - 1 ? r.len : min(r.len, r.lo + chunk);
+  if (r.lo >= r.hi && r.split > 0) r.any = false;  // (range 0 is always written)
+  return r;
+}
+__device__ __forceinline__ u32x4_t query_bits(u32x4_t w, const AttnArgs& a) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ a.q_flip) & a.q_keep;
+  return w;
+}
+
+// The base of a column's powers of two is moved only once a score is 2^8 above it: the sums stay far from f32's end, and the outputs are
+// rescaled a few times a range instead of every step
+constexpr float kSlack = 8.f;
 
 // max and sum over the four groups of sixteen lanes, in every lane
 __device__ __forceinline__ float groups_max(float v) {
@@ -48,6 +87,42 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// What some rows of the step see of a token and earlier ones do not (the causal edge) must not reach the earlier ones, and a product
+// with a zero would let an infinity or a NaN through. So such values are zero for the product, and the end of the kernel adds them to
+// the rows that see them, which are infinite or NaN by them whatever else they hold. What no row sees is zero.
+template <bool F8>
+__device__ __forceinline__ bool is_wild(uint32_t half_or_byte) {
+  return F8 ? (half_or_byte & 0x7Fu) == 0x7Fu : (half_or_byte & 0x7F80u) == 0x7F80u;
+}
+// a lane's words of a token's V: zero if `out`; at the causal edge (`edge`) without what is infinite or NaN, and whether there was any
+template <bool F8, int N>
+__device__ __forceinline__ bool clean_v(uint32_t (&w)[N], bool out, bool edge) {
+  constexpr uint32_t bits = F8 ? 8 : 16, mask = F8 ? 0xFFu : 0xFFFFu;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (out) w[i] = 0u;
+#pragma unroll
+    for (uint32_t b = 0; b < 32; b += bits)
+      if (edge && is_wild<F8>(w[i] >> b)) odd = true, w[i] &= ~(mask << b);
+  }
+  return odd;
+}
+// value d of a token's V if it is infinite or NaN, else 0
+template <bool F8>
+__device__ __forceinline__ float wild_value(const uint8_t* v, int d) {
+  if (F8) return is_wild<true>(v[d]) ? __builtin_nanf("") : 0.f;
+  const uint32_t b = reinterpret_cast<const uint16_t*>(v)[d];
+  return is_wild<false>(b) ? bf16_bits_to_f32(b) : 0.f;
+}
+// own or prefix token t of a head's pool; null if its page does not exist
+template <bool F8>
+__device__ __forceinline__ const uint8_t* token_at(const AttnArgs& a, const int32_t* tab, const uint8_t* pool, int t) {
+  const int page = tab[t >> a.page_shift];
+  if (page < 0 || page >= a.c.npages) return nullptr;
+  return pool + ((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * (F8 ? 1 : 2);
+}
 
 // ---- one wave, sixteen query columns, thirty-two tokens a step, nothing through LDS ----------------------------------------------
 // Scores are S[token][query] = K Q^T by v_mfma_f32_16x16x32_bf16: a lane brings one token's (lane % 16) sixteen bytes a step of the
@@ -65,6 +140,7 @@ struct Narrow {
   v8bf_t q[NS];
   v4f_t o[VL];
   float m, l;
+  bool odd;  // see clean_v
 
   struct Block {
     u32x4_t k[2][KW];
@@ -72,18 +148,18 @@ struct Narrow {
   };
 
   __device__ __forceinline__ void begin() {
-    m = -__builtin_inff(), l = 0.f;
+    m = -__builtin_inff(), l = 0.f, odd = false;
 #pragma unroll
     for (int i = 0; i < VL; ++i) o[i] = v4f_t{0.f, 0.f, 0.f, 0.f};
   }
   // row: the lane's query (lane % 16), D values; null: none
-  __device__ __forceinline__ void load_q(const uint16_t* row, int g) {
+  __device__ __forceinline__ void load_q(const uint16_t* row, int g, const AttnArgs& a) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
       u32x4_t w = {0, 0, 0, 0};
       if (row) w = *reinterpret_cast<const DSGX_GLOBAL u32x4_t*>((uintptr_t)(row + d));
-      q[s] = __builtin_bit_cast(v8bf_t, w);
+      q[s] = __builtin_bit_cast(v8bf_t, query_bits(w, a));
     }
   }
   // kp, vp: the pools at the two tiles' first tokens (wave-uniform); ts: bytes from token to token
@@ -136,17 +212,8 @@ struct Narrow {
     }
     lo = __builtin_bit_cast(v8bf_t, a), hi = __builtin_bit_cast(v8bf_t, b);
   }
-  // Whether a V word holds an infinity or a NaN
-  __device__ __forceinline__ static bool wild(uint32_t w) {
-    if (F8) {
-      const uint32_t n = w & 0x7F7F7F7Fu;
-      return ((n + 0x01010101u) & 0x80808080u) != 0;  // a byte of 0x7F
-    }
-    return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-  }
-
-  // Thirty-two tokens, t0 the first. lim: the lane's query sees the tokens below it. there[a]: tile a's page exists. all: no lane has
-  // anything masked here (wave-uniform). seen: some query's tokens end at `seen` at most; step rows' limits run from lim_lo to seen.
+  // Thirty-two tokens, t0 the first. lim: the lane's query sees the tokens below it. there0, there1: the tiles' pages exist. all: no lane
+  // has anything masked here (wave-uniform). The rows' limits run from lim_lo to seen.
   __device__ __forceinline__ void step(Block& x, int t0, int lim, bool there0, bool there1, bool all, int lim_lo, int seen, float s2, int lane) {
     const int g = lane >> 4;
     v4f_t s[2];
@@ -158,70 +225,39 @@ struct Narrow {
     }
     float e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = __fmul_rn(s[i / 4][i % 4], s2);
-    bool odd = false;
+    for (int i = 0; i < 8; ++i) e[i] = s[i / 4][i % 4];
     if (!all) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
         const bool there = i < 4 ? there0 : there1;
         if (!there || t >= lim) e[i] = -__builtin_inff();
-        // what no query sees is zero for the product (0 * NaN); what some do and some do not is looked at below
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          if (!there || t >= seen) x.v[i][w] = 0u;
-          odd |= t >= lim_lo && wild(x.v[i][w]);
-        }
+        odd |= clean_v<F8, VW>(x.v[i], !there || t >= seen, t >= lim_lo);
       }
     }
     float mx = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-    mx = fmaxf(m, groups_max(mx));
-    const float base = mx == -__builtin_inff() ? 0.f : mx;
-    const float alpha = exp2_hw(m - base);
-    m = mx;
+    mx = __fmul_rn(groups_max(mx), s2);
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {  // (-inf + slack: the first scores move it)
+      const float to = fmaxf(m, mx), alpha = exp2_hw(m - (to == -__builtin_inff() ? 0.f : to));
+      l *= alpha, m = to;
+#pragma unroll
+      for (int i = 0; i < VL; ++i) o[i] *= alpha;
+    }
+    const float base = m == -__builtin_inff() ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = exp2_hw(e[i] - base), sum += e[i];
-    l = fmaf(l, alpha, sum);
+    for (int i = 0; i < 8; ++i) e[i] = exp2_hw(fmaf(e[i], s2, -base)), sum += e[i];
+    l += sum;
     const u32x4_t pw = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
     const v8bf_t p = __builtin_bit_cast(v8bf_t, pw);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) o[i] *= alpha;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) == 0, 1)) {
-#pragma unroll
-      for (int i = 0; i < VL; i += 2) {
-        v8bf_t a, b;
-        v_operands(x.v, i, a, b);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p, o[i], 0, 0, 0);
-        o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p, o[i + 1], 0, 0, 0);
-      }
-    } else {
-      // A token that one row of the step sees and an earlier one does not holds an infinity or a NaN: the rows one limit at a time,
-      // from the last to the first, each with the tokens past its limit zeroed
-      for (int lm = seen; lm >= lim_lo; --lm) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t0 + 16 * (i / 4) + 4 * g + i % 4 >= lm) {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) x.v[i][w] = 0u;
-          }
-        const bool mine = lim == lm;
-#pragma unroll
-        for (int i = 0; i < VL; i += 2) {
-          v8bf_t a, b;
-          v_operands(x.v, i, a, b);
-          const v4f_t n0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p, o[i], 0, 0, 0), n1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p, o[i + 1], 0, 0, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = mine ? n0[j] : o[i][j], o[i + 1][j] = mine ? n1[j] : o[i + 1][j];
-        }
-      }
+    for (int i = 0; i < VL; i += 2) {
+      v8bf_t a, b;
+      v_operands(x.v, i, a, b);
+      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p, o[i], 0, 0, 0);
+      o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p, o[i + 1], 0, 0, 0);
     }
   }
-};
-
-// The rows that attend over one set of tokens, as query columns: column x is head h G + x % G of row first + x / G
-struct Columns {
-  int first, count;  // rows; columns in all
 };
 
 template <int D, bool F8>
@@ -230,23 +266,10 @@ __global__ void __launch_bounds__(256) k_attn_narrow(AttnArgs a, int prefix) {
   constexpr int VL = N::VL, LD = D + 4;
   extern __shared__ float lds[];  // [4][16][LD] outputs, then [4][16] maxima and sums
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
-  const int h = blockIdx.x % a.c.Hkv, split = blockIdx.x / a.c.Hkv, G = a.G;
-  int first = 0, rows = a.b.rows, len = a.b.prefix_len;
-  const int32_t* tab = a.b.prefix;
-  if (!prefix) {
-    const int b = blockIdx.z;
-    first = a.b.cu_rows ? a.b.cu_rows[b] : b * a.b.max_rows;
-    const int end = a.b.cu_rows ? a.b.cu_rows[b + 1] : first + a.b.max_rows;
-    if (first < 0 || end <= first || end > a.b.rows) return;
-    rows = end - first;
-    const int cap = a.b.table_ld << a.page_shift;
-    len = a.b.lens[b];
-    len = len < 0 ? 0 : len > cap ? cap : len;
-    tab = a.b.table + (size_t)b * a.b.table_ld;
-  }
-  const int chunk = prefix ? a.p.cp : a.p.co, splits = prefix ? a.p.sp : a.p.so;
-  const int lo = split * chunk, hi = split == splits - 1 ? len : min(len, lo + chunk);
-  if (lo >= hi && split > 0) return;  // (range 0 is always written)
+  const Range rg = range_of(a, prefix);
+  if (!rg.any) return;
+  const int h = rg.head, split = rg.split, rows = rg.rows, len = rg.len, lo = rg.lo, hi = rg.hi, first = rg.first, G = a.G;
+  const int32_t* tab = rg.tab;
   const bool direct = a.p.sp + a.p.so == 1;
   const int esz = F8 ? 1 : 2;
   const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
@@ -264,7 +287,7 @@ __global__ void __launch_bounds__(256) k_attn_narrow(AttnArgs a, int prefix) {
     const int lim_lo = prefix ? len : len - rows + (tile * 16) / G + 1, lim_hi = prefix ? len : len - rows + last + 1;
     N n;
     n.begin();
-    n.load_q(live ? a.q + (size_t)(first + row) * a.ldq + (size_t)head * D : nullptr, g);
+    n.load_q(live ? a.q + (size_t)(first + row) * a.ldq + (size_t)head * D : nullptr, g, a);
     const int stop = min(hi, lim_hi);
 
     auto fetch = [&](typename N::Block& blk, int t0, bool& there0, bool& there1) {
@@ -293,7 +316,19 @@ __global__ void __launch_bounds__(256) k_attn_narrow(AttnArgs a, int prefix) {
       cur = nxt, c0 = n0, c1 = n1;
     }
 
-    // the four waves' halves of the answer joined
+    if (__builtin_amdgcn_ballot_w64(n.odd)) {
+#pragma unroll 1
+      for (int t = max(lo, lim_lo); t < stop; ++t) {
+        if ((((t - lo) >> 5) & 3) != wave) continue;
+        const uint8_t* v = token_at<F8>(a, tab, vh, t);
+        if (!v || t >= min(lim, hi)) continue;
+#pragma unroll
+        for (int i = 0; i < VL; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) n.o[i][j] += wild_value<F8>(v, VL * (4 * g + j) + i);
+      }
+    }
+    // the four waves' parts of the answer joined
     n.l = groups_sum(n.l);
     __syncthreads();
 #pragma unroll
@@ -334,6 +369,320 @@ __global__ void __launch_bounds__(256) k_attn_narrow(AttnArgs a, int prefix) {
   }
 }
 
+// ---- four waves, QW query columns each, tiles of 8192 / D tokens through LDS -------------------------------------------------------
+// For many columns over the same tokens (the prefix under a batch, 64 heads over one) the matrix unit is the time, and a token's K and V
+// are read by four waves. A tile is staged through registers: e4m3 becomes bf16 there, and V is transposed there (four tokens by eight
+// values a thread, a byte permutation a pair), so that both operands are 16-byte reads from LDS. Layouts (chunks of 16 bytes): K as rows of
+// a token, V as rows of a d whose chunks hold the eight tokens that one lane's scores belong to, so that the scores are the second
+// product's operand as they stand; the chunks of a row are XORed with its number, which spreads sixteen lanes' rows over all banks.
+// QW 32: v_mfma_f32_32x32x16_bf16, 128 columns a workgroup; QW 16: v_mfma_f32_16x16x32_bf16, 64 columns.
+typedef float v16f_t __attribute__((ext_vector_type(16)));
+
+template <int D, bool F8, int QW>
+struct Wide {
+  static constexpr int KV = 8192 / D;            // tokens a tile
+  static constexpr int SR = QW / 16 * 4 * (QW / 16);  // accumulators of a tile a lane: 16 or 4
+  static constexpr int LG = kWave / QW;          // lanes that share a column: 2 or 4
+  static constexpr int KD = 8 * LG;              // k of one instruction: 16 or 32
+  static constexpr int NS = D / KD, ST = KV / QW, OT = D / QW, NE = KV * QW / kWave, NP = NE / 8;
+  static constexpr int KN = F8 ? 2 : 4, VW = F8 ? 2 : 4;
+  static constexpr int kTile = 16384;            // bytes of a tile of K, of V
+  using acc_t = typename std::conditional<QW == 32, v16f_t, v4f_t>::type;
+
+  __device__ __forceinline__ static acc_t mfma(v8bf_t a, v8bf_t b, acc_t c) {
+    if constexpr (QW == 32) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  // the token (in its tile) of a lane's score i, the d of its result i in output tile t
+  __device__ __forceinline__ static int token_of(int i, int lg) {
+    return QW == 32 ? 32 * (i / 16) + 8 * ((i % 16) / 4) + 4 * lg + i % 4 : 16 * (i / 4) + 4 * lg + i % 4;
+  }
+  __device__ __forceinline__ static uint32_t k_addr(uint32_t row, uint32_t c) {
+    constexpr uint32_t CPR = D / 8;  // chunks a row
+    if (D == 64) return row / 2 * 256 + (row & 1) * 128 + ((c ^ (row >> 1)) & 7) * 16;
+    return row * (CPR * 16) + (c ^ (row & 15)) * 16;
+  }
+  __device__ __forceinline__ static uint32_t v_addr(uint32_t d, uint32_t c) {
+    constexpr uint32_t CPR = KV / 8, RP = 16 / CPR;  // chunks a row, rows of 256 bytes
+    return d * (CPR * 16) + ((c ^ (d / RP) ^ (d >> 4)) & (CPR - 1)) * 16;
+  }
+
+  // The operands' reads as the lane's address XOR a constant, plus a constant: row QW u + col, chunk LG k + lg of a tile of K ..
+  __device__ __forceinline__ static uint32_t k_read(uint32_t lane_at, int u, int k) { return (lane_at ^ (uint32_t)(LG * k * 16)) + (uint32_t)(QW * u * D * 2); }
+  // .. and row QW i + col, chunk LG k + lg of one of V^T (the row's share of the XOR that i makes is i's alone: no carries)
+  __device__ __forceinline__ static uint32_t v_read(uint32_t lane_at, int i, int k) {
+    constexpr uint32_t CPR = KV / 8, RP = 16 / CPR;
+    const uint32_t x = (uint32_t)(LG * k) ^ ((uint32_t)(QW * i / RP) & (CPR - 1)) ^ ((uint32_t)(QW * i / 16) & (CPR - 1));
+    return (lane_at ^ (x * 16)) + (uint32_t)(QW * i) * (CPR * 16);
+  }
+
+  struct Stage {
+    u32x4_t k[KN];
+    uint32_t v[4][VW];
+  };
+  // the sixteens of tokens that a thread's loads lie in: K's load i, V's
+  __device__ __forceinline__ static uint32_t k_row(int i, uint32_t tid) { return (tid + 256 * i) / (F8 ? D / 16 : D / 8); }
+  __device__ __forceinline__ static uint32_t k_chunk(int i, uint32_t tid) { return (tid + 256 * i) % (F8 ? D / 16 : D / 8); }
+  __device__ __forceinline__ static uint32_t v_group(uint32_t tid) { return tid / (D / 8); }  // of four tokens
+
+  // at: byte offsets of the tile's sixteens (lane s % 16 .. of `offs`), from the head's first value
+  __device__ __forceinline__ static void load(Stage& x, const uint8_t* kh, const uint8_t* vh, uint64_t offs, uint32_t ts, uint32_t tid) {
+    auto off = [&](uint32_t sixteen) {
+      const uint32_t lo = __shfl((int)(uint32_t)offs, (int)sixteen), hi = __shfl((int)(offs >> 32), (int)sixteen);
+      return (uint64_t)hi << 32 | lo;
+    };
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const uint32_t row = k_row(i, tid);
+      x.k[i] = *(const DSGX_GLOBAL u32x4_t*)(uintptr_t)(kh + off(row / 16) + (row % 16) * ts + 16 * k_chunk(i, tid));
+    }
+    const uint32_t grp = v_group(tid), dc = tid % (D / 8);
+    const uint8_t* vb = vh + off(grp / 4) + (grp % 4) * 4 * ts + dc * VW * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (F8) {
+        const u32x2_t t = *(const DSGX_GLOBAL u32x2_t*)(uintptr_t)(vb + j * ts);
+        x.v[j][0] = t[0], x.v[j][1] = t[1];
+      } else {
+        const u32x4_t t = *(const DSGX_GLOBAL u32x4_t*)(uintptr_t)(vb + j * ts);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[j][i] = t[i];
+      }
+    }
+  }
+  // tokens 4 grp .. + 3: their chunk of a row of V^T and the half of it
+  __device__ __forceinline__ static uint32_t v_chunk(uint32_t grp) { return QW == 32 ? 2 * (grp / 4) + (grp & 1) : 4 * (grp / 8) + (grp & 3); }
+  __device__ __forceinline__ static uint32_t v_half(uint32_t grp) { return QW == 32 ? (grp >> 1) & 1 : (grp >> 2) & 1; }
+  __device__ __forceinline__ static void store(const Stage& x, uint8_t* kt, uint8_t* vt, uint32_t tid) {
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const uint32_t row = k_row(i, tid), c = k_chunk(i, tid);
+      if constexpr (F8) {
+        uint32_t w[4];
+        fp8x8_to_bf16(x.k[i][0], x.k[i][1], w);
+        *reinterpret_cast<u32x4_t*>(kt + k_addr(row, 2 * c)) = u32x4_t{w[0], w[1], w[2], w[3]};
+        fp8x8_to_bf16(x.k[i][2], x.k[i][3], w);
+        *reinterpret_cast<u32x4_t*>(kt + k_addr(row, 2 * c + 1)) = u32x4_t{w[0], w[1], w[2], w[3]};
+      } else {
+        *reinterpret_cast<u32x4_t*>(kt + k_addr(row, c)) = x.k[i];
+      }
+    }
+    const uint32_t grp = v_group(tid), dc = tid % (D / 8), chunk = v_chunk(grp), half = v_half(grp);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {  // d = 8 dc + i and the next
+      u32x2_t a, b;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (F8) {
+          const uint32_t w = __builtin_amdgcn_perm(x.v[2 * h + 1][i / 4], x.v[2 * h][i / 4], i % 4 ? 0x07030602u : 0x05010400u);
+          a[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+          b[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+        } else {
+          a[h] = __builtin_amdgcn_perm(x.v[2 * h + 1][i / 2], x.v[2 * h][i / 2], 0x05040100u);
+          b[h] = __builtin_amdgcn_perm(x.v[2 * h + 1][i / 2], x.v[2 * h][i / 2], 0x07060302u);
+        }
+      }
+      *reinterpret_cast<u32x2_t*>(vt + v_addr(8 * dc + i, chunk) + 8 * half) = a;
+      *reinterpret_cast<u32x2_t*>(vt + v_addr(8 * dc + i + 1, chunk) + 8 * half) = b;
+    }
+  }
+};
+
+// max and sum over the lanes that share a column
+template <int QW>
+__device__ __forceinline__ float column_max(float v) {
+  if (QW == 16) return groups_max(v);
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int QW>
+__device__ __forceinline__ float column_sum(float v) {
+  if (QW == 16) return groups_sum(v);
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D, bool F8, int QW>
+__global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide(AttnArgs a, int prefix) {
+  using W = Wide<D, F8, QW>;
+  using acc_t = typename W::acc_t;
+  constexpr int KV = W::KV, COLS = 4 * QW, NE = W::NE;
+  extern __shared__ __align__(16) uint8_t tiles[];  // two tiles of K and V each
+  __shared__ int any_odd;
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const int wave = uni((int)tid >> 6), lg = lane / QW, col = lane % QW;
+  const Range rg = range_of(a, prefix);
+  if (!rg.any) return;
+  const int h = rg.head, split = rg.split, rows = rg.rows, len = rg.len, lo = rg.lo, hi = rg.hi, first = rg.first, G = a.G;
+  const int32_t* tab = rg.tab;
+  constexpr int esz = F8 ? 1 : 2;
+  const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
+  const uint8_t *kh = static_cast<const uint8_t*>(a.c.k) + h * a.c.head_stride * esz, *vh = static_cast<const uint8_t*>(a.c.v) + h * a.c.head_stride * esz;
+  const float s2 = F8 ? a.scale2 * a.c.ks[h] : a.scale2, vs = F8 ? a.c.vs[h] : 1.f;
+
+  const int cols = rows * G;
+  for (int tile = blockIdx.y; tile * COLS < cols; tile += gridDim.y) {
+    const int x = tile * COLS + wave * QW + col, row = x / G, head = h * G + x % G;
+    const bool live = x < cols;
+    const int last = min(tile * COLS + COLS - 1, cols - 1) / G;
+    const int lim_hi = prefix ? len : len - rows + last + 1, stop = min(hi, lim_hi);
+    const int lim_lo = min(hi, prefix ? len : len - rows + tile * COLS / G + 1);
+    const int lim = !live ? 0 : min(hi, prefix ? len : len - rows + row + 1);
+    v8bf_t q[W::NS];
+#pragma unroll
+    for (int s = 0; s < W::NS; ++s) {
+      u32x4_t w = {0, 0, 0, 0};
+      if (live) w = *reinterpret_cast<const DSGX_GLOBAL u32x4_t*>((uintptr_t)(a.q + (size_t)(first + row) * a.ldq + (size_t)head * D + W::KD * s + 8 * lg));
+      q[s] = __builtin_bit_cast(v8bf_t, query_bits(w, a));
+    }
+    acc_t o[W::OT];
+#pragma unroll
+    for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+      for (int j = 0; j < W::SR; ++j) o[i][j] = 0.f;
+    float m = -__builtin_inff(), l = 0.f;  // m: the base, in scores; l: this lane's part of the sum
+
+    // lane s < KV / 16: the page of the sixteen s of a tile, and where it lies
+    auto page_of = [&](int t0) {
+      const int t = t0 + 16 * (int)lane;
+      return (int)lane < KV / 16 && t < stop ? tab[t >> a.page_shift] : -1;
+    };
+    auto place = [&](int t0, int page, uint32_t& there) {
+      const int t = t0 + 16 * (int)lane;
+      const bool ok = page >= 0 && page < a.c.npages;
+      there = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+      return ok ? (uint64_t)(((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * esz) : 0ull;
+    };
+    constexpr uint32_t kAll = (1u << (KV / 16)) - 1;
+    bool odd = false;  // see clean_v
+    auto clean = [&](typename W::Stage& st, int t0, uint32_t there) {
+      const uint32_t grp = W::v_group(tid);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = t0 + 4 * (int)grp + j;
+        odd |= clean_v<F8, W::VW>(st.v[j], !(there >> (grp / 4) & 1) || t >= stop, t >= lim_lo);
+      }
+    };
+
+    typename W::Stage st;
+    uint32_t there = 0, next_there = 0;
+    int page = page_of(lo), ahead = page_of(lo + KV);
+    __syncthreads();  // (the tiles of a column tile before this one have been read)
+    if (lo < stop) {
+      const uint64_t at = place(lo, page, there);
+      W::load(st, kh, vh, at, ts, tid);
+      if (there != kAll || lo + KV > lim_lo) clean(st, lo, there);
+      W::store(st, tiles, tiles + W::kTile, tid);
+    }
+    const uint32_t k_at = W::k_addr(col, lg), v_at = W::v_addr(col, lg);
+    int buf = 0;
+    for (int t0 = lo; t0 < stop; t0 += KV, buf ^= 1) {
+      __syncthreads();
+      const bool more = t0 + KV < stop;
+      if (more) {
+        const uint64_t at = place(t0 + KV, ahead, next_there);
+        W::load(st, kh, vh, at, ts, tid);
+        ahead = page_of(t0 + 2 * KV);
+      }
+      const uint8_t *kt = tiles + buf * 2 * W::kTile, *vt = kt + W::kTile;
+      uint32_t ka = k_at, va = v_at;
+      asm volatile("" : "+v"(ka), "+v"(va));  // (else every operand's address is kept in a register of its own)
+      float e[NE];
+#pragma unroll
+      for (int u = 0; u < W::ST; ++u) {
+        acc_t s;
+#pragma unroll
+        for (int j = 0; j < W::SR; ++j) s[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < W::NS; ++k)
+          s = W::mfma(__builtin_bit_cast(v8bf_t, *reinterpret_cast<const u32x4_t*>(kt + W::k_read(ka, u, k))), q[k], s);
+#pragma unroll
+        for (int j = 0; j < W::SR; ++j) e[u * W::SR + j] = s[j];
+      }
+      const bool all = there == kAll && t0 + KV <= lim_lo;
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          const int tk = W::token_of(i, lg);
+          if (!(there >> (tk / 16) & 1) || t0 + tk >= lim) e[i] = -__builtin_inff();
+        }
+      }
+      float mx = e[0];
+#pragma unroll
+      for (int i = 1; i < NE; ++i) mx = fmaxf(mx, e[i]);
+      mx = __fmul_rn(column_max<QW>(mx), s2);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {  // (-inf + slack: the first scores move it)
+        const float to = fmaxf(m, mx), base = to == -__builtin_inff() ? 0.f : to, alpha = exp2_hw(m - base);
+        l *= alpha, m = to;
+#pragma unroll
+        for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+          for (int j = 0; j < W::SR; ++j) o[i][j] *= alpha;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) e[i] = exp2_hw(fmaf(e[i], s2, -base)), sum += e[i];
+      l += sum;
+      v8bf_t p[W::NP];
+#pragma unroll
+      for (int k = 0; k < W::NP; ++k) {
+        const u32x4_t pw = {pack_bf16(e[8 * k], e[8 * k + 1]), pack_bf16(e[8 * k + 2], e[8 * k + 3]), pack_bf16(e[8 * k + 4], e[8 * k + 5]), pack_bf16(e[8 * k + 6], e[8 * k + 7])};
+        p[k] = __builtin_bit_cast(v8bf_t, pw);
+      }
+#pragma unroll
+      for (int k = 0; k < W::NP; ++k)
+#pragma unroll
+        for (int i = 0; i < W::OT; ++i) o[i] = W::mfma(__builtin_bit_cast(v8bf_t, *reinterpret_cast<const u32x4_t*>(vt + W::v_read(va, i, k))), p[k], o[i]);
+      if (more) {
+        if (next_there != kAll || t0 + 2 * KV > lim_lo) clean(st, t0 + KV, next_there);
+        uint8_t* nt = tiles + (buf ^ 1) * 2 * W::kTile;
+        W::store(st, nt, nt + W::kTile, tid);
+        there = next_there;
+      }
+    }
+
+    l = column_sum<QW>(l);
+    if (lim_lo < stop) {  // (wave-uniform, and the same for all waves)
+      if (tid == 0) any_odd = 0;
+      __syncthreads();
+      if (odd) any_odd = 1;
+      __syncthreads();
+      if (any_odd) {
+#pragma unroll 1
+        for (int t = max(lo, lim_lo); t < stop; ++t) {
+          const uint8_t* v = token_at<F8>(a, tab, vh, t);
+          if (!v || t >= lim) continue;
+#pragma unroll
+          for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+            for (int j = 0; j < W::SR; ++j) o[i][j] += wild_value<F8>(v, QW * i + W::LG * (j & ~3) + 4 * lg + (j & 3));
+        }
+      }
+    }
+    if (!live) continue;
+    const size_t rh = (size_t)(first + row) * a.Hq + head;
+    if (a.p.sp + a.p.so == 1) {
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
+      uint16_t* dst = a.out + (size_t)(first + row) * a.ldo + (size_t)head * D;
+#pragma unroll
+      for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+        for (int j = 0; j < W::SR; j += 4)
+          *reinterpret_cast<uint2*>(dst + QW * i + W::LG * j + 4 * lg) = make_uint2(pack_bf16(o[i][j] * inv, o[i][j + 1] * inv), pack_bf16(o[i][j + 2] * inv, o[i][j + 3] * inv));
+      if (lg == 0 && a.lse) a.lse[rh] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    } else {
+      const size_t slot = (size_t)((prefix ? 0 : a.p.sp) + split) * a.b.rows * a.Hq + rh;
+      float* dst = a.part + slot * D;
+#pragma unroll
+      for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+        for (int j = 0; j < W::SR; j += 4) *reinterpret_cast<v4f_t*>(dst + QW * i + W::LG * j + 4 * lg) = v4f_t{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]};
+      if (lg == 0) a.ml[slot] = make_float2(m, l);
+    }
+  }
+}
+
 // One wave a row's head: the ranges' outputs joined by their maxima
 template <int D>
 __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
@@ -369,32 +718,46 @@ __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
 
 int round_up(int64_t v, int m) { return (int)((v + m - 1) / m * m); }
 
+// How a set of tokens is worked on by `cols` query columns: sixteen of them a workgroup, or tiles through LDS for 64 or 128
+enum Kind { kNarrow, kWide16, kWide32 };
+Kind kind_of(int64_t cols) {
+  return cols <= 16 ? kNarrow : cols <= 64 ? kWide16 : kWide32;
+}
+int cols_of(Kind k) { return k == kNarrow ? 16 : k == kWide16 ? 64 : 128; }
+
 Plan make_plan(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
   const int G = Hq / c.Hkv, cus = num_cus_cached();
-  auto cut = [&](int64_t len, int64_t tiles, int& n, int& chunk) {  // tiles: workgroups a range
-    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / std::max<int64_t>(1, tiles));
+  auto cut = [&](int64_t len, int64_t cols, int64_t sets, int& n, int& chunk) {
+    const Kind k = kind_of(cols);
+    const int64_t tiles = sets * c.Hkv * ((cols + cols_of(k) - 1) / cols_of(k));  // workgroups a range
+    const int64_t want = std::max<int64_t>(1, (k == kNarrow ? 4 : 2) * (int64_t)cus / std::max<int64_t>(1, tiles));
     chunk = std::max(256, round_up((len + want - 1) / want, 128));
     n = (int)std::max<int64_t>(1, (len + chunk - 1) / chunk);
   };
   Plan p{0, 128, 1, 128};
-  if (b.prefix_len) cut(b.prefix_len, (int64_t)c.Hkv * (((int64_t)b.rows * G + 15) / 16), p.sp, p.cp);
-  cut(b.max_len, (int64_t)c.Hkv * b.B * (((int64_t)b.max_rows * G + 15) / 16), p.so, p.co);
+  if (b.prefix_len) cut(b.prefix_len, (int64_t)b.rows * G, 1, p.sp, p.cp);
+  cut(b.max_len, (int64_t)b.max_rows * G, b.B, p.so, p.co);
   return p;
 }
 size_t ml_bytes(const Plan& p, const dsgx_kv_batch& b, int Hq) { return align256((size_t)(p.sp + p.so) * b.rows * Hq * sizeof(float2)); }
 
 template <int D, bool F8>
-int launch(const AttnArgs& a, hipStream_t st) {
-  const size_t lds = (4 * 16 * (D + 4) + 128) * 4;
-  auto kern = k_attn_narrow<D, F8>;
+int launch_part(const AttnArgs& a, int prefix, hipStream_t st) {
+  const int64_t cols = (int64_t)(prefix ? a.b.rows : a.b.max_rows) * a.G;
+  const Kind k = kind_of(cols);
+  const size_t lds = k == kNarrow ? (4 * 16 * (D + 4) + 128) * 4 : 4 * Wide<D, F8, 32>::kTile;
+  auto kern = k == kNarrow ? k_attn_narrow<D, F8> : k == kWide16 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
   if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
-  auto tiles = [&](int64_t rows) { return (unsigned)std::min<int64_t>(65535, (rows * a.G + 15) / 16); };
-  if (a.p.sp) {
-    hipLaunchKernelGGL(kern, dim3(a.p.sp * a.c.Hkv, tiles(a.b.rows)), dim3(256), lds, st, a, 1);
-    DSGX_HIP(hipGetLastError());
-  }
-  hipLaunchKernelGGL(kern, dim3(a.p.so * a.c.Hkv, tiles(a.b.max_rows), a.b.B), dim3(256), lds, st, a, 0);
+  const dim3 grid((prefix ? a.p.sp : a.p.so) * a.c.Hkv, (unsigned)std::min<int64_t>(65535, (cols + cols_of(k) - 1) / cols_of(k)), prefix ? 1 : a.b.B);
+  hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a, prefix);
   DSGX_HIP(hipGetLastError());
+  return DSGX_OK;
+}
+template <int D, bool F8>
+int launch(const AttnArgs& a, hipStream_t st) {
+  if (a.p.sp)
+    if (int rc = launch_part<D, F8>(a, 1, st)) return rc;
+  if (int rc = launch_part<D, F8>(a, 0, st)) return rc;
   if (a.p.sp + a.p.so > 1) {
     hipLaunchKernelGGL(k_combine<D>, dim3(a.b.rows, (a.Hq + 3) / 4), dim3(256), 0, st, a);
     DSGX_HIP(hipGetLastError());
@@ -426,6 +789,7 @@ extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch,
                          float* lse, void* ws, void* stream) {
   if (int rc = check(cache, batch, Hq)) return rc;
   if (!q || !out || !ws) return fail(DSGX_EINVAL, "attn: null queries, output or workspace");
+  if (!std::isfinite(scale)) return fail(DSGX_EINVAL, "attn: a scale of %g", (double)scale);
   const int64_t vals = (int64_t)Hq * cache->D;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)ws) & 15 || ldq % 8 || ldo % 8 || ldq < vals || ldo < vals)
     return fail(DSGX_EINVAL, "attn: rows %lld, %lld apart (multiples of 8, %lld at least; 16-byte aligned)", (long long)ldq, (long long)ldo, (long long)vals);
@@ -433,7 +797,7 @@ extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch,
   AttnArgs a{};
   a.c = *cache, a.b = *batch, a.p = make_plan(*cache, *batch, Hq);
   a.q = q, a.out = out, a.lse = lse, a.ldq = ldq, a.ldo = ldo, a.Hq = Hq, a.G = Hq / cache->Hkv, a.page_shift = __builtin_ctz((unsigned)cache->page);
-  a.scale2 = scale * kLog2e;
+  a.scale2 = scale == 0.f ? 1.f : std::fabs(scale) * kLog2e, a.q_flip = scale < 0.f ? 0x80008000u : 0u, a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu;
   a.ml = static_cast<float2*>(ws);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ml_bytes(a.p, *batch, Hq));
   hipStream_t st = static_cast<hipStream_t>(stream);
