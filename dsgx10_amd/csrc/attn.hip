@@ -19,50 +19,157 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
-struct Plan {
-  int sp, cp;  // ranges of the prefix, tokens a range
-  int so, co;  // ranges of a sequence's own tokens, tokens a range
+// How the work is cut. The prefix: `splits` ranges of `chunk` tokens, `tiles` tiles of `cols` query columns of all rows. The sequences' own
+// tokens: ranges of a length that the kernels find from lens when they run (own_plan), so that about `target` workgroups have the same to do
+// whatever max_len announced; at most `most` of them have a place for what they leave.
+// A workgroup has `heads` heads of keys and values side by side (1, 2 or 4, a divisor of Hkv; own: as many at most).
+struct Part {
+  int cols, tiles, splits, chunk, heads;  // the prefix
+};
+struct Own {
+  int cols, target, least, most, heads;  // least: tokens a range at least (a multiple of 128)
 };
 struct AttnArgs {
   dsgx_kv_cache c;
   dsgx_kv_batch b;
-  Plan p;
+  Part pre;
+  Own own;
   const uint16_t* q;
   uint16_t* out;
-  float *lse, *part;
-  float2* ml;
+  float *lse, *part;  // part: [places][cols][D], the prefix's first
+  float2* ml;         // [places][cols]
   int64_t ldq, ldo;
   int Hq, G, page_shift;
   float scale2;              // |scale| log2 e; 1 for a scale of zero
   uint32_t q_flip, q_keep;   // the scale's sign and whether it is zero, on the queries' bits
 };
 
-// The tokens and rows of a workgroup: a range of the prefix for all rows, or of a sequence's own tokens for its rows
-struct Range {
-  const int32_t* tab;
-  int head, split, first, rows, len, lo, hi;  // lo .. hi - 1 of len tokens
-  bool any;
+#define DSGX_CONST __attribute__((address_space(4)))  // read-only while a kernel runs: uniform loads go to the scalar unit
+typedef const DSGX_CONST int32_t* table_t;
+
+// A lane's sequence of 64 from j0 on: its rows, its own tokens, its tiles of `cols` columns
+struct Seq {
+  int first, rows, len, tiles;
 };
-__device__ __forceinline__ Range range_of(const AttnArgs& a, int prefix) {
-  Range r{a.b.prefix, (int)blockIdx.x % a.c.Hkv, (int)blockIdx.x / a.c.Hkv, 0, a.b.rows, a.b.prefix_len, 0, 0, true};
-  if (!prefix) {
-    const int b = blockIdx.z;
-    r.first = a.b.cu_rows ? a.b.cu_rows[b] : b * a.b.max_rows;
-    const int end = a.b.cu_rows ? a.b.cu_rows[b + 1] : r.first + a.b.max_rows;
-    if (r.first < 0 || end <= r.first || end > a.b.rows) {
-      r.any = false;
-      return r;
-    }
-    r.rows = end - r.first;
-    const int cap = a.b.table_ld << a.page_shift, len = a.b.lens[b];
-    r.len = len < 0 ? 0 : len > cap ? cap : len;
-    r.tab = a.b.table + (size_t)b * a.b.table_ld;
-  }
-  const int chunk = prefix ? a.p.cp : a.p.co, splits = prefix ? a.p.sp : a.p.so;
-  r.lo = r.split * chunk, r.hi = r.split == splits - 1 ? r.len : min(r.len, r.lo + chunk);
-  if (r.lo >= r.hi && r.split > 0) r.any = false;  // (range 0 is always written)
-  return r;
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int j) {
+  Seq s{0, 0, 0, 0};
+  if (j >= a.b.B) return s;
+  const int lo = a.b.cu_rows ? a.b.cu_rows[j] : j * a.b.max_rows, hi = a.b.cu_rows ? a.b.cu_rows[j + 1] : lo + a.b.max_rows, len = a.b.lens[j];
+  if (lo < 0 || hi <= lo || hi > a.b.rows) return s;
+  const int cap = a.b.table_ld << a.page_shift;
+  s.first = lo, s.rows = hi - lo, s.len = len < 0 ? 0 : len > cap ? cap : len;
+  s.tiles = (s.rows * a.G + a.own.cols - 1) / a.own.cols;
+  return s;
 }
+// inclusive sums over the lanes: DPP shifts within the rows of sixteen, then the rows' last lanes handed on
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3
+  return scan_step<0x143, 0xC>(v);  // row_bcast 31 into rows 2 and 3
+}
+__device__ __forceinline__ int ranges_of(const Seq& s, int chunk) { return s.len ? (s.len + chunk - 1) / chunk : 1; }
+// Tokens a range of the sequences' own, by a whole wave; s: the lane's sequence of the first 64. The kernels that ask get the same answer.
+// A workgroup does a whole number of ranges one after the other: for one to four of them, ranges just long enough that there are no more of
+// them (each sequence's last one is short) than workgroups times that, and of the four the choice that is done first, a range's own
+// cost (set-up, joining) being that of kRangeCost tokens.
+// Heads side by side are worth their longer way through the tokens (a wave has its head's alone) while that is 96 tokens or more.
+constexpr int kRangeCost = 192, kTogether = 96;
+struct Cut {
+  int chunk, heads;
+};
+__device__ __forceinline__ Cut own_plan(const AttnArgs& a, const Seq& s, int lane) {
+  if (a.own.target == 0) return Cut{1 << 30, 1};  // a range a sequence
+  float w = (float)s.tiles * (float)s.len;
+  for (int j0 = kWave; j0 < a.b.B; j0 += kWave) {
+    const Seq t = seq_of(a, j0 + lane);
+    w += (float)t.tiles * (float)t.len;
+  }
+  w = uni(wave_sum(w)) * (float)a.c.Hkv * 1.0001f;
+  int heads = a.own.heads, best = 0;
+  while (heads > 1 && w < (float)a.own.target * (float)(kTogether * heads)) heads >>= 1;
+  const float groups = (float)(a.c.Hkv / heads);
+  w /= (float)heads;
+  float cost = 3e38f;
+#pragma unroll 1
+  for (int turns = 1; turns <= 4; ++turns) {
+    const float room = (float)(a.own.target * turns);
+    int chunk = max(heads > 1 ? 128 : a.own.least, ((int)min(w / room, 1e9f) + 128) & ~127);
+    float all = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < 3; ++k) {
+      int n = s.tiles * ranges_of(s, chunk);
+      for (int j0 = kWave; j0 < a.b.B; j0 += kWave) {
+        const Seq t = seq_of(a, j0 + lane);
+        n += t.tiles * ranges_of(t, chunk);
+      }
+      all = uni(wave_sum((float)n)) * groups;
+      if (all <= room) break;
+      if (k < 2) chunk = ((int)min((float)chunk * all / room, 1e9f) + 128) & ~127;
+    }
+    const float c = ceilf(all / (float)a.own.target) * (float)(chunk + kRangeCost);
+    if (c < cost) cost = c, best = chunk;
+  }
+  return Cut{best, heads};
+}
+// The sequence that `item` (of all sequences' ranges times tiles) falls to, and how many items precede the sequence's; false past the last
+__device__ __forceinline__ bool own_find(const AttnArgs& a, const Seq& s0, int chunk, int item, int lane, Seq& s, int& b, int& before) {
+  int run = 0;
+  for (int j0 = 0; j0 < a.b.B; j0 += kWave) {
+    const Seq t = j0 ? seq_of(a, j0 + lane) : s0;
+    const int mine = t.tiles * ranges_of(t, chunk), upto = run + wave_scan(mine);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > item);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      b = j0 + l, before = __builtin_amdgcn_readlane(upto - mine, l);
+      s = Seq{__builtin_amdgcn_readlane(t.first, l), __builtin_amdgcn_readlane(t.rows, l), __builtin_amdgcn_readlane(t.len, l), __builtin_amdgcn_readlane(t.tiles, l)};
+      return true;
+    }
+    run = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// What a workgroup works on: tile `tile` of the columns of rows first .. first + rows - 1, over tokens lo .. hi - 1 of len, with the heads
+// from `head` on
+struct Item {
+  table_t tab;
+  int head, first, rows, len, lo, hi, tile;
+  int64_t place, next;  // of the first head's first column in part and ml, and from a head to the next
+  bool causal, alone;   // alone: nobody else adds to these columns, so that the result is final
+};
+// (the compiler cannot know that what came out of a search over the lanes is the same in all of them)
+__device__ __forceinline__ int64_t uni64(int64_t v) { return (int64_t)((uint64_t)uni((uint32_t)((uint64_t)v >> 32)) << 32 | uni((uint32_t)v)); }
+__device__ __forceinline__ Item uniform(const Item& t) {
+  return Item{(table_t)uni64((int64_t)t.tab), uni(t.head), uni(t.first), uni(t.rows), uni(t.len), uni(t.lo), uni(t.hi), uni(t.tile), uni64(t.place), uni64(t.next), uni((int)t.causal) != 0,
+              uni((int)t.alone) != 0};
+}
+__device__ __forceinline__ Item prefix_item(const AttnArgs& a, bool& any) {
+  // The tiles that read the same tokens run on the same XCD (workgroup i runs on XCD i % 8) next to each other, out of its L2
+  const int i = blockIdx.x, pair = i / 8 / a.pre.tiles * 8 + i % 8, groups = a.c.Hkv / a.pre.heads, split = pair / groups;
+  Item t{(table_t)(uintptr_t)a.b.prefix, pair % groups * a.pre.heads, 0, a.b.rows, a.b.prefix_len, split * a.pre.chunk, 0, i / 8 % a.pre.tiles, 0, 0, false, false};
+  t.hi = min(t.len, t.lo + a.pre.chunk), t.next = (int64_t)a.pre.tiles * a.pre.cols;
+  t.place = (int64_t)(split * a.c.Hkv + t.head) * t.next + (int64_t)t.tile * a.pre.cols;
+  any = split < a.pre.splits;
+  return t;
+}
+__device__ __forceinline__ int64_t own_places(const AttnArgs& a) { return (int64_t)a.pre.splits * a.c.Hkv * a.pre.tiles * a.pre.cols; }
+__device__ __forceinline__ bool own_item(const AttnArgs& a, const Seq& s0, Cut cut, int item, int lane, Item& t) {
+  Seq s;
+  int b, before;
+  const int chunk = cut.chunk, groups = a.c.Hkv / cut.heads;
+  if (!own_find(a, s0, chunk, item / groups, lane, s, b, before)) return false;
+  const int n = item / groups, i = n - before, split = i / s.tiles, head = item % groups * cut.heads;
+  if ((int64_t)(n + 1) * a.c.Hkv > a.own.most) return false;
+  t = Item{(table_t)(uintptr_t)(a.b.table + (size_t)b * a.b.table_ld), head, s.first, s.rows, s.len, split * chunk, (int)min((int64_t)s.len, (int64_t)(split + 1) * chunk), i % s.tiles,
+           own_places(a) + ((int64_t)n * a.c.Hkv + head) * a.own.cols, a.own.cols, true, a.pre.splits == 0 && ranges_of(s, chunk) == 1};
+  return true;
+}
+
 __device__ __forceinline__ u32x4_t query_bits(u32x4_t w, const AttnArgs& a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ a.q_flip) & a.q_keep;
@@ -95,18 +202,16 @@ template <bool F8>
 __device__ __forceinline__ bool is_wild(uint32_t half_or_byte) {
   return F8 ? (half_or_byte & 0x7Fu) == 0x7Fu : (half_or_byte & 0x7F80u) == 0x7F80u;
 }
-// a lane's words of a token's V: zero if `out`; at the causal edge (`edge`) without what is infinite or NaN, and whether there was any
+// a lane's words of a token's V without what is infinite or NaN if the token lies at the edge, and whether there was any
 template <bool F8, int N>
-__device__ __forceinline__ bool clean_v(uint32_t (&w)[N], bool out, bool edge) {
+__device__ __forceinline__ bool clean_edge(uint32_t (&w)[N], bool edge) {
   constexpr uint32_t bits = F8 ? 8 : 16, mask = F8 ? 0xFFu : 0xFFFFu;
   bool odd = false;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (out) w[i] = 0u;
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (uint32_t b = 0; b < 32; b += bits)
       if (edge && is_wild<F8>(w[i] >> b)) odd = true, w[i] &= ~(mask << b);
-  }
   return odd;
 }
 // value d of a token's V if it is infinite or NaN, else 0
@@ -118,7 +223,7 @@ __device__ __forceinline__ float wild_value(const uint8_t* v, int d) {
 }
 // own or prefix token t of a head's pool; null if its page does not exist
 template <bool F8>
-__device__ __forceinline__ const uint8_t* token_at(const AttnArgs& a, const int32_t* tab, const uint8_t* pool, int t) {
+__device__ __forceinline__ const uint8_t* token_at(const AttnArgs& a, table_t tab, const uint8_t* pool, int t) {
   const int page = tab[t >> a.page_shift];
   if (page < 0 || page >= a.c.npages) return nullptr;
   return pool + ((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * (F8 ? 1 : 2);
@@ -130,17 +235,23 @@ __device__ __forceinline__ const uint8_t* token_at(const AttnArgs& a, const int3
 // (lane % 16). O[d][query] = V^T P: the same eight scores of a lane (two tiles of sixteen tokens) are the P operand as they are, and
 // the V operand is eight tokens' values of one d, which a lane picks out of the eight rows it loaded (a whole row of V is sixteen lanes):
 // one byte permutation a pair. The d that a tile's row stands for is VL (lane % 16) + tile: a lane's results are contiguous.
-template <int D, bool F8>
+// neither the compiler's passes nor its scheduler move a load across
+__device__ __forceinline__ void loads_stay() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int D, bool F8, int NQ>
 struct Narrow {
   static constexpr int NS = D / 32;               // steps of the score product
   static constexpr int VL = D / 16;               // values of a row of V a lane
   static constexpr int KW = F8 ? D / 64 : D / 32;  // 16-byte words of a row of K a lane
   static constexpr int VW = F8 ? VL / 4 : VL / 2;  // 32-bit words of a row of V a lane
 
-  v8bf_t q[NS];
-  v4f_t o[VL];
-  float m, l;
-  bool odd;  // see clean_v
+  v8bf_t q[NQ][NS];
+  v4f_t o[NQ][VL];
+  float m[NQ], l[NQ];
+  bool odd;  // see clean_edge
 
   struct Block {
     u32x4_t k[2][KW];
@@ -148,47 +259,53 @@ struct Narrow {
   };
 
   __device__ __forceinline__ void begin() {
-    m = -__builtin_inff(), l = 0.f, odd = false;
+    odd = false;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) o[i] = v4f_t{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NQ; ++n) {
+      m[n] = -__builtin_inff(), l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < VL; ++i) o[n][i] = v4f_t{0.f, 0.f, 0.f, 0.f};
+    }
   }
-  // row: the lane's query (lane % 16), D values; null: none
-  __device__ __forceinline__ void load_q(const uint16_t* row, int g, const AttnArgs& a) {
+  // row: the lane's query (lane % 16) of set n, D values; null: none
+  __device__ __forceinline__ void load_q(int n, const uint16_t* row, int g, const AttnArgs& a) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int d = F8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
       u32x4_t w = {0, 0, 0, 0};
       if (row) w = *reinterpret_cast<const DSGX_GLOBAL u32x4_t*>((uintptr_t)(row + d));
-      q[s] = __builtin_bit_cast(v8bf_t, query_bits(w, a));
+      q[n][s] = __builtin_bit_cast(v8bf_t, query_bits(w, a));
     }
   }
-  // kp, vp: the pools at the two tiles' first tokens (wave-uniform); ts: bytes from token to token
-  __device__ __forceinline__ static void load(Block& x, const uint8_t* const (&kp)[2], const uint8_t* const (&vp)[2], uint32_t ts, int lane) {
-    const uint32_t c = lane & 15, g = lane >> 4;
-    const uint32_t ko = c * ts + 16 * g, vo = 4 * g * ts + c * VW * 4;
+  // p0, p1: a pool at the two tiles' first tokens (wave-uniform); ko, vo: the lane's offsets, ts: bytes from token to token
+  __device__ __forceinline__ static void load_k(Block& x, const uint8_t* p0, const uint8_t* p1, uint32_t ko) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int j = 0; j < KW; ++j) x.k[a][j] = ldg_stream(kp[a], ko + 64 * j);
+      for (int j = 0; j < KW; ++j) x.k[a][j] = ldg_stream(a ? p1 : p0, ko + 64 * j);
+  }
+  __device__ __forceinline__ static void load_v(Block& x, const uint8_t* p0, const uint8_t* p1, uint32_t vo, uint32_t ts) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        const uint8_t* p = a ? p1 : p0;
         const uint32_t at = vo + j * ts;
         uint32_t(&w)[VW] = x.v[4 * a + j];
         if constexpr (VW >= 4) {
 #pragma unroll
           for (int h = 0; h < VW / 4; ++h) {
-            const u32x4_t t = ldg_stream(vp[a], at + 16 * h);
+            const u32x4_t t = ldg_stream(p, at + 16 * h);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[4 * h + i] = t[i];
           }
         } else if constexpr (VW == 2) {
-          const u32x2_t t = __builtin_nontemporal_load((const DSGX_GLOBAL u32x2_t*)((const DSGX_GLOBAL uint8_t*)(uintptr_t)vp[a] + at));
+          const u32x2_t t = __builtin_nontemporal_load((const DSGX_GLOBAL u32x2_t*)((const DSGX_GLOBAL uint8_t*)(uintptr_t)p + at));
           w[0] = t[0], w[1] = t[1];
         } else {
-          w[0] = __builtin_nontemporal_load((const DSGX_GLOBAL uint32_t*)((const DSGX_GLOBAL uint8_t*)(uintptr_t)vp[a] + at));
+          w[0] = __builtin_nontemporal_load((const DSGX_GLOBAL uint32_t*)((const DSGX_GLOBAL uint8_t*)(uintptr_t)p + at));
         }
       }
-    }
   }
   __device__ __forceinline__ static v8bf_t k_operand(const u32x4_t (&k)[KW], int s) {
     if (!F8) return __builtin_bit_cast(v8bf_t, k[s]);
@@ -212,160 +329,232 @@ struct Narrow {
     }
     lo = __builtin_bit_cast(v8bf_t, a), hi = __builtin_bit_cast(v8bf_t, b);
   }
-  // Thirty-two tokens, t0 the first. lim: the lane's query sees the tokens below it. there0, there1: the tiles' pages exist. all: no lane
-  // has anything masked here (wave-uniform). The rows' limits run from lim_lo to seen.
-  __device__ __forceinline__ void step(Block& x, int t0, int lim, bool there0, bool there1, bool all, int lim_lo, int seen, float s2, int lane) {
-    const int g = lane >> 4;
-    v4f_t s[2];
+  __device__ __forceinline__ void scores(const Block& x, float (&e)[NQ][8]) const {
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      s[a] = v4f_t{0.f, 0.f, 0.f, 0.f};
+      v4f_t s[NQ];
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_operand(x.k[a], i), q[i], s[a], 0, 0, 0);
+      for (int n = 0; n < NQ; ++n) s[n] = v4f_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const v8bf_t k = k_operand(x.k[a], i);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][i], s[n], 0, 0, 0);
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[n][4 * a + i] = s[n][i];
     }
-    float e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = s[i / 4][i % 4];
+  }
+  // Scores of thirty-two tokens from t0 on to the softmax's numerators, as the second product's operand. lim: the lane's query sees the
+  // tokens below it; there0, there1: the tiles' pages exist; all: no lane has anything masked here (wave-uniform)
+  __device__ __forceinline__ v8bf_t softmax(int n, float (&e)[8], int t0, int lim, bool there0, bool there1, bool all, float s2, int g) {
     if (!all) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
-        const bool there = i < 4 ? there0 : there1;
-        if (!there || t >= lim) e[i] = -__builtin_inff();
-        odd |= clean_v<F8, VW>(x.v[i], !there || t >= seen, t >= lim_lo);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (!(i < 4 ? there0 : there1) || t0 + 16 * (i / 4) + 4 * g + i % 4 >= lim) e[i] = -__builtin_inff();
     }
     float mx = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
     mx = __fmul_rn(groups_max(mx), s2);
-    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {  // (-inf + slack: the first scores move it)
-      const float to = fmaxf(m, mx), alpha = exp2_hw(m - (to == -__builtin_inff() ? 0.f : to));
-      l *= alpha, m = to;
+    if (__builtin_amdgcn_ballot_w64(mx > m[n] + kSlack)) {  // (-inf + slack: the first scores move it)
+      const float to = fmaxf(m[n], mx), alpha = exp2_hw(m[n] - (to == -__builtin_inff() ? 0.f : to));
+      l[n] *= alpha, m[n] = to;
 #pragma unroll
-      for (int i = 0; i < VL; ++i) o[i] *= alpha;
+      for (int i = 0; i < VL; ++i) o[n][i] *= alpha;
     }
-    const float base = m == -__builtin_inff() ? 0.f : m;
+    const float base = m[n] == -__builtin_inff() ? 0.f : m[n];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = exp2_hw(fmaf(e[i], s2, -base)), sum += e[i];
-    l += sum;
+    l[n] += sum;
     const u32x4_t pw = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
-    const v8bf_t p = __builtin_bit_cast(v8bf_t, pw);
+    return __builtin_bit_cast(v8bf_t, pw);
+  }
+  // what no query sees is zero for the product; the rows' limits run from lim_lo to seen
+  __device__ __forceinline__ void clean(Block& x, int t0, bool there0, bool there1, int lim_lo, int seen, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
+      const bool out = !(i < 4 ? there0 : there1) || t >= seen;
+#pragma unroll
+      for (int w = 0; w < VW; ++w) x.v[i][w] = out ? 0u : x.v[i][w];
+      if (lim_lo < seen) odd |= clean_edge<F8, VW>(x.v[i], t >= lim_lo);
+    }
+  }
+  __device__ __forceinline__ void add(const Block& x, const v8bf_t (&p)[NQ]) {
 #pragma unroll
     for (int i = 0; i < VL; i += 2) {
       v8bf_t a, b;
       v_operands(x.v, i, a, b);
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p, o[i], 0, 0, 0);
-      o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p, o[i + 1], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[n], o[n][i], 0, 0, 0);
+        o[n][i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p[n], o[n][i + 1], 0, 0, 0);
+      }
     }
   }
 };
 
-template <int D, bool F8>
-__global__ void __launch_bounds__(256) k_attn_narrow(AttnArgs a, int prefix) {
-  using N = Narrow<D, F8>;
-  constexpr int VL = N::VL, LD = D + 4;
-  extern __shared__ float lds[];  // [4][16][LD] outputs, then [4][16] maxima and sums
-  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
-  const Range rg = range_of(a, prefix);
-  if (!rg.any) return;
-  const int h = rg.head, split = rg.split, rows = rg.rows, len = rg.len, lo = rg.lo, hi = rg.hi, first = rg.first, G = a.G;
-  const int32_t* tab = rg.tab;
-  const bool direct = a.p.sp + a.p.so == 1;
-  const int esz = F8 ? 1 : 2;
-  const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
-  const uint8_t *kh = static_cast<const uint8_t*>(a.c.k) + h * a.c.head_stride * esz, *vh = static_cast<const uint8_t*>(a.c.v) + h * a.c.head_stride * esz;
-  const float s2 = F8 ? a.scale2 * a.c.ks[h] : a.scale2, vs = F8 ? a.c.vs[h] : 1.f;
-  float* red = lds + 4 * 16 * LD;
+// Waves a SIMD that the registers leave room for, and blocks on their way a wave
+template <int D, bool F8, int NQ>
+constexpr int kNarrowWaves = D == 64 ? 3 : D == 128 ? 2 : F8 ? 2 : 1;
+template <int D, bool F8, int NQ>
+constexpr int kNarrowDepth = D == 64 ? (NQ == 2 ? 1 : F8 ? 3 : 2) : D == 128 ? (F8 ? (NQ == 1 ? 3 : 2) : NQ == 1 ? 2 : 1) : 1;
 
-  const int cols = rows * G;
-  for (int tile = blockIdx.y; tile * 16 < cols; tile += gridDim.y) {
-    const int x = tile * 16 + col, row = x / G, head = h * G + x % G;
-    const bool live = x < cols;
-    const int lim = !live ? 0 : prefix ? len : len - rows + row + 1;
-    // the limits of the tile's first and last row
-    const int last = min(tile * 16 + 15, cols - 1) / G;
-    const int lim_lo = prefix ? len : len - rows + (tile * 16) / G + 1, lim_hi = prefix ? len : len - rows + last + 1;
+template <int D, bool F8, int NQ>
+__global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(AttnArgs a, int prefix) {
+  using N = Narrow<D, F8, NQ>;
+  constexpr int VL = N::VL, LD = D + 4, COLS = 16 * NQ;
+  extern __shared__ float lds[];  // [4][COLS][LD] outputs, then [4][COLS] maxima and sums
+  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), g = lane >> 4, col = lane & 15, G = a.G;
+  constexpr int esz = F8 ? 1 : 2;
+  const uint32_t ts = (uint32_t)(a.c.tok_stride * esz), ko = col * ts + 16 * g, vo = 4 * g * ts + col * N::VW * 4;
+  float *red_m = lds + 4 * COLS * LD, *red_l = red_m + 4 * COLS;
+  Seq s0{};
+  Cut cut{0, a.pre.heads};
+  if (!prefix) s0 = seq_of(a, lane), cut = own_plan(a, s0, lane);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    Item it;
+    if (prefix) {
+      bool any;
+      it = prefix_item(a, any);
+      if (!any) return;
+    } else if (!own_item(a, s0, cut, item, lane, it)) {
+      return;
+    }
+    it = uniform(it);
+    const int heads = uni(cut.heads), wph = 4 / heads, step = 32 * wph;  // waves a head, which share its tokens
+    const int h = it.head + wave / wph, len = it.len, rows = it.rows, cols = rows * G, x0 = it.tile * COLS;
+    const uint8_t *kh = static_cast<const uint8_t*>(a.c.k) + h * a.c.head_stride * esz, *vh = static_cast<const uint8_t*>(a.c.v) + h * a.c.head_stride * esz;
+    const float s2 = F8 ? a.scale2 * a.c.ks[h] : a.scale2;
+    // the limits of the tile's first and last row, and of the lane's
+    const int lim_hi = it.causal ? len - rows + min(x0 + COLS - 1, cols - 1) / G + 1 : len, stop = min(it.hi, lim_hi);
+    const int lim_lo = min(it.hi, it.causal ? len - rows + x0 / G + 1 : len);
     N n;
     n.begin();
-    n.load_q(live ? a.q + (size_t)(first + row) * a.ldq + (size_t)head * D : nullptr, g, a);
-    const int stop = min(hi, lim_hi);
-
-    auto fetch = [&](typename N::Block& blk, int t0, bool& there0, bool& there1) {
-      const uint8_t *kp[2], *vp[2];
-      bool th[2];
+    int lim[NQ];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = t0 + 16 * i;
-        int page = -1;
-        if (t < stop) page = uni(tab[t >> a.page_shift]);
-        th[i] = page >= 0 && page < a.c.npages;
-        const int64_t at = th[i] ? ((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * esz : 0;
-        kp[i] = kh + at, vp[i] = vh + at;
-      }
-      there0 = th[0], there1 = th[1];
-      N::load(blk, kp, vp, ts, lane);
-    };
-    typename N::Block cur, nxt;
-    bool c0 = false, c1 = false, n0 = false, n1 = false;
-    int t0 = lo + 32 * wave;
-    if (t0 < stop) fetch(cur, t0, c0, c1);
-    for (; t0 < stop; t0 += 128) {
-      if (t0 + 128 < stop) fetch(nxt, t0 + 128, n0, n1);
-      const bool all = c0 && c1 && t0 + 32 <= lim_lo && t0 + 32 <= stop;
-      n.step(cur, t0, min(lim, hi), c0, c1, all, min(lim_lo, hi), stop, s2, lane);
-      cur = nxt, c0 = n0, c1 = n1;
+    for (int k = 0; k < NQ; ++k) {
+      const int x = x0 + 16 * k + col, row = x / G;
+      const bool live = x < cols;
+      lim[k] = !live ? 0 : min(it.hi, it.causal ? len - rows + row + 1 : len);
+      n.load_q(k, live ? a.q + (size_t)(it.first + row) * a.ldq + (size_t)(h * G + x % G) * D : nullptr, g, a);
     }
 
+    auto page_of = [&](int t) { return t < stop ? it.tab[t >> a.page_shift] : -1; };
+    auto place = [&](int t, int page, bool& there) -> int64_t {  // bytes from a head's first value
+      there = page >= 0 && page < a.c.npages;
+      return there ? ((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * esz : 0;
+    };
+    // DEPTH blocks of tokens are on their way, each in registers of its own: a block's K registers are loaded again as soon as its scores are
+    // there, its V registers after its product. The page numbers are read a step before
+    constexpr int DEPTH = kNarrowDepth<D, F8, NQ>;
+    typename N::Block blk[DEPTH];
+    bool c0[DEPTH], c1[DEPTH];
+    int t0 = it.lo + 32 * (wave % wph);
+    if (t0 < stop) {
+      int64_t at0 = 0, at1 = 0;
+#pragma unroll
+      for (int s = 0; s < DEPTH; ++s) {
+        const int t = t0 + step * s;
+        const int64_t n0 = place(t, page_of(t), c0[s]), n1 = place(t + 16, page_of(t + 16), c1[s]);
+        const bool in = t < stop;  // (else one line of the block before)
+        at0 = in ? n0 : at0, at1 = in ? n1 : at1;
+        const uint32_t ks = in ? ko : 0u, vo_s = in ? vo : 0u, ts_s = in ? ts : 0u;
+        N::load_k(blk[s], kh + at0, kh + at1, ks);
+        loads_stay();  // (issued in the loop's order, or its waits are for more than they need)
+        N::load_v(blk[s], vh + at0, vh + at1, vo_s, ts_s);
+        loads_stay();
+      }
+      int ahead0 = page_of(t0 + step * DEPTH), ahead1 = page_of(t0 + step * DEPTH + 16);
+      // (no way out between the blocks of a turn: it would make the waits at the turn's start those of the shortest way there)
+      for (; t0 < stop; t0 += step * DEPTH) {
+#pragma unroll
+        for (int s = 0; s < DEPTH; ++s) {
+          const int t = t0 + step * s, tn = t + step * DEPTH;
+          const bool more = tn < stop, all = c0[s] && c1[s] && t + 32 <= lim_lo;
+          bool n0 = false, n1 = false;
+          // (after the last block the registers are loaded from one line of it: every turn issues the same loads)
+          if (more) at0 = place(tn, ahead0, n0), at1 = place(tn + 16, ahead1, n1);
+          const uint32_t kn = more ? ko : 0u, vn = more ? vo : 0u, tsn = more ? ts : 0u;
+          float e[NQ][8];
+          n.scores(blk[s], e);
+          loads_stay();
+          N::load_k(blk[s], kh + at0, kh + at1, kn);
+          ahead0 = page_of(tn + step), ahead1 = page_of(tn + step + 16);
+          loads_stay();
+          if (s == 0 || t < stop) {
+            v8bf_t p[NQ];
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) p[k] = n.softmax(k, e[k], t, lim[k], c0[s], c1[s], all, s2, g);
+            if (!all) n.clean(blk[s], t, c0[s], c1[s], lim_lo, stop, g);
+            n.add(blk[s], p);
+          }
+          loads_stay();
+          N::load_v(blk[s], vh + at0, vh + at1, vn, tsn);
+          loads_stay();
+          c0[s] = n0, c1[s] = n1;
+        }
+      }
+    }
     if (__builtin_amdgcn_ballot_w64(n.odd)) {
 #pragma unroll 1
-      for (int t = max(lo, lim_lo); t < stop; ++t) {
-        if ((((t - lo) >> 5) & 3) != wave) continue;
-        const uint8_t* v = token_at<F8>(a, tab, vh, t);
-        if (!v || t >= min(lim, hi)) continue;
+      for (int t = max(it.lo, lim_lo); t < stop; ++t) {
+        if (((t - it.lo) >> 5) % wph != wave % wph) continue;
+        const uint8_t* v = token_at<F8>(a, it.tab, vh, t);
+        if (!v) continue;
 #pragma unroll
-        for (int i = 0; i < VL; ++i)
+        for (int k = 0; k < NQ; ++k)
+          if (t < lim[k]) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) n.o[i][j] += wild_value<F8>(v, VL * (4 * g + j) + i);
+            for (int i = 0; i < VL; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) n.o[k][i][j] += wild_value<F8>(v, VL * (4 * g + j) + i);
+          }
       }
     }
+
     // the four waves' parts of the answer joined
-    n.l = groups_sum(n.l);
+    __syncthreads();  // (what an item before this one left has been read)
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) {
+      const int c = wave * COLS + 16 * k + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m4 = 0; m4 < VL; m4 += 4)
+          *reinterpret_cast<v4f_t*>(lds + c * LD + VL * (4 * g + i) + m4) = v4f_t{n.o[k][m4][i], n.o[k][m4 + 1][i], n.o[k][m4 + 2][i], n.o[k][m4 + 3][i]};
+      const float l = groups_sum(n.l[k]);
+      if (g == 0) red_m[c] = n.m[k], red_l[c] = l;
+    }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int m4 = 0; m4 < VL; m4 += 4)
-        *reinterpret_cast<v4f_t*>(lds + (wave * 16 + col) * LD + VL * (4 * g + i) + m4) = v4f_t{n.o[m4][i], n.o[m4 + 1][i], n.o[m4 + 2][i], n.o[m4 + 3][i]};
-    if (g == 0) red[wave * 16 + col] = n.m, red[64 + wave * 16 + col] = n.l;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-      const int qc = i / (D / 4), d = 4 * (i % (D / 4)), xx = tile * 16 + qc;
-      if (xx >= cols) continue;
-      float mm = -__builtin_inff(), w[4], l = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mm = fmaxf(mm, red[k * 16 + qc]);
+    for (int i = threadIdx.x; i < heads * COLS * (D / 4); i += 256) {
+      const int c = i / (D / 4) % COLS, hd = i / (COLS * (D / 4)), d = 4 * (i % (D / 4)), x = x0 + c, w0 = hd * wph;
+      if (x >= cols) continue;
+      float mm = -__builtin_inff(), l = 0.f;
+      for (int k = w0; k < w0 + wph; ++k) mm = fmaxf(mm, red_m[k * COLS + c]);
       const float base = mm == -__builtin_inff() ? 0.f : mm;
       v4f_t acc = {0.f, 0.f, 0.f, 0.f};
+      for (int k = w0; k < w0 + wph; ++k) {
+        const float w = exp2_hw(red_m[k * COLS + c] - base);
+        l = fmaf(w, red_l[k * COLS + c], l);
+        const v4f_t v = *reinterpret_cast<const v4f_t*>(lds + (k * COLS + c) * LD + d);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        w[k] = exp2_hw(red[k * 16 + qc] - base);
-        l = fmaf(w[k], red[64 + k * 16 + qc], l);
-        const v4f_t v = *reinterpret_cast<const v4f_t*>(lds + (k * 16 + qc) * LD + d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = fmaf(w[k], v[j], acc[j]);
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(w, v[j], acc[j]);
       }
-      const size_t rh = (size_t)(first + xx / G) * a.Hq + h * G + xx % G;
-      if (direct) {
-        const float inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
-        *reinterpret_cast<uint2*>(a.out + (size_t)(first + xx / G) * a.ldo + (size_t)(h * G + xx % G) * D + d) =
-            make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-        if (d == 0 && a.lse) a.lse[rh] = l == 0.f ? -__builtin_inff() : (mm + __builtin_amdgcn_logf(l)) * kLn2;
+      if (it.alone) {
+        const int row = it.first + x / G, head = (it.head + hd) * G + x % G;
+        const float vs = F8 ? a.c.vs[it.head + hd] : 1.f, inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
+        *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)head * D + d) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+        if (d == 0 && a.lse) a.lse[(size_t)row * a.Hq + head] = l == 0.f ? -__builtin_inff() : (mm + __builtin_amdgcn_logf(l)) * kLn2;
       } else {
-        const size_t slot = (size_t)((prefix ? 0 : a.p.sp) + split) * a.b.rows * a.Hq + rh;
-        *reinterpret_cast<v4f_t*>(a.part + slot * D + d) = acc;
-        if (d == 0) a.ml[slot] = make_float2(mm, l);
+        const int64_t at = it.place + hd * it.next + c;
+        *reinterpret_cast<v4f_t*>(a.part + at * D + d) = acc;
+        if (d == 0) a.ml[at] = make_float2(mm, l);
       }
     }
+    if (prefix) return;
   }
 }
 
@@ -511,23 +700,30 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
   __shared__ int any_odd;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const int wave = uni((int)tid >> 6), lg = lane / QW, col = lane % QW;
-  const Range rg = range_of(a, prefix);
-  if (!rg.any) return;
-  const int h = rg.head, split = rg.split, rows = rg.rows, len = rg.len, lo = rg.lo, hi = rg.hi, first = rg.first, G = a.G;
-  const int32_t* tab = rg.tab;
   constexpr int esz = F8 ? 1 : 2;
   const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
-  const uint8_t *kh = static_cast<const uint8_t*>(a.c.k) + h * a.c.head_stride * esz, *vh = static_cast<const uint8_t*>(a.c.v) + h * a.c.head_stride * esz;
-  const float s2 = F8 ? a.scale2 * a.c.ks[h] : a.scale2, vs = F8 ? a.c.vs[h] : 1.f;
-
-  const int cols = rows * G;
-  for (int tile = blockIdx.y; tile * COLS < cols; tile += gridDim.y) {
-    const int x = tile * COLS + wave * QW + col, row = x / G, head = h * G + x % G;
+  Seq s0{};
+  Cut cut{0, a.pre.heads};
+  if (!prefix) s0 = seq_of(a, lane), cut = own_plan(a, s0, lane);
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    Item it;
+    if (prefix) {
+      bool any;
+      it = prefix_item(a, any);
+      if (!any) return;
+    } else if (!own_item(a, s0, cut, item, lane, it)) {
+      return;
+    }
+    it = uniform(it);
+    const int h = it.head, len = it.len, rows = it.rows, G = a.G, cols = rows * G, x0 = it.tile * COLS, lo = it.lo, first = it.first;
+    const table_t tab = it.tab;
+    const uint8_t *kh = static_cast<const uint8_t*>(a.c.k) + h * a.c.head_stride * esz, *vh = static_cast<const uint8_t*>(a.c.v) + h * a.c.head_stride * esz;
+    const float s2 = F8 ? a.scale2 * a.c.ks[h] : a.scale2, vs = F8 ? a.c.vs[h] : 1.f;
+    const int x = x0 + wave * QW + col, row = x / G, head = h * G + x % G;
     const bool live = x < cols;
-    const int last = min(tile * COLS + COLS - 1, cols - 1) / G;
-    const int lim_hi = prefix ? len : len - rows + last + 1, stop = min(hi, lim_hi);
-    const int lim_lo = min(hi, prefix ? len : len - rows + tile * COLS / G + 1);
-    const int lim = !live ? 0 : min(hi, prefix ? len : len - rows + row + 1);
+    const int lim_hi = it.causal ? len - rows + min(x0 + COLS - 1, cols - 1) / G + 1 : len, stop = min(it.hi, lim_hi);
+    const int lim_lo = min(it.hi, it.causal ? len - rows + x0 / G + 1 : len);
+    const int lim = !live ? 0 : min(it.hi, it.causal ? len - rows + row + 1 : len);
     v8bf_t q[W::NS];
 #pragma unroll
     for (int s = 0; s < W::NS; ++s) {
@@ -554,13 +750,16 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
       return ok ? (uint64_t)(((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * esz) : 0ull;
     };
     constexpr uint32_t kAll = (1u << (KV / 16)) - 1;
-    bool odd = false;  // see clean_v
+    bool odd = false;  // see clean_edge
     auto clean = [&](typename W::Stage& st, int t0, uint32_t there) {
       const uint32_t grp = W::v_group(tid);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int t = t0 + 4 * (int)grp + j;
-        odd |= clean_v<F8, W::VW>(st.v[j], !(there >> (grp / 4) & 1) || t >= stop, t >= lim_lo);
+        const bool out = !(there >> (grp / 4) & 1) || t >= stop;
+#pragma unroll
+        for (int w = 0; w < W::VW; ++w) st.v[j][w] = out ? 0u : st.v[j][w];
+        if (lim_lo < stop) odd |= clean_edge<F8, W::VW>(st.v[j], t >= lim_lo);
       }
     };
 
@@ -660,9 +859,7 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
         }
       }
     }
-    if (!live) continue;
-    const size_t rh = (size_t)(first + row) * a.Hq + head;
-    if (a.p.sp + a.p.so == 1) {
+    if (live && it.alone) {
       const float inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
       uint16_t* dst = a.out + (size_t)(first + row) * a.ldo + (size_t)head * D;
 #pragma unroll
@@ -670,98 +867,176 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
 #pragma unroll
         for (int j = 0; j < W::SR; j += 4)
           *reinterpret_cast<uint2*>(dst + QW * i + W::LG * j + 4 * lg) = make_uint2(pack_bf16(o[i][j] * inv, o[i][j + 1] * inv), pack_bf16(o[i][j + 2] * inv, o[i][j + 3] * inv));
-      if (lg == 0 && a.lse) a.lse[rh] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
-    } else {
-      const size_t slot = (size_t)((prefix ? 0 : a.p.sp) + split) * a.b.rows * a.Hq + rh;
-      float* dst = a.part + slot * D;
+      if (lg == 0 && a.lse) a.lse[(size_t)(first + row) * a.Hq + head] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    } else if (live) {
+      const int64_t at = it.place + wave * QW + col;
+      float* dst = a.part + at * D;
 #pragma unroll
       for (int i = 0; i < W::OT; ++i)
 #pragma unroll
         for (int j = 0; j < W::SR; j += 4) *reinterpret_cast<v4f_t*>(dst + QW * i + W::LG * j + 4 * lg) = v4f_t{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]};
-      if (lg == 0) a.ml[slot] = make_float2(m, l);
+      if (lg == 0) a.ml[at] = make_float2(m, l);
     }
+    if (prefix) return;
   }
 }
 
-// One wave a row's head: the ranges' outputs joined by their maxima
-template <int D>
+// The ranges' outputs of a row's head joined by their maxima: WPH waves a head, D / 4 lanes a range
+template <int D, int WPH>
 __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
-  constexpr int PL = D / 64;
-  const int lane = threadIdx.x & 63, r = blockIdx.x, head = uni((int)(blockIdx.y * 4 + (threadIdx.x >> 6)));
-  if (head >= a.Hq) return;
-  const RowPlace p = find_row(a.b, r, lane);
-  if (p.seq < 0 || p.end > a.b.rows) return;
-  const int cap = a.b.table_ld << a.page_shift, len = p.len < 0 ? 0 : p.len > cap ? cap : p.len;
-  const int own = max(1, min(a.p.so, (len + a.p.co - 1) / a.p.co)), ns = a.p.sp + own;
-  const size_t per = (size_t)a.b.rows * a.Hq, rh = (size_t)r * a.Hq + head;
-  float mm = -__builtin_inff();
-  for (int s = lane; s < ns; s += kWave) mm = fmaxf(mm, a.ml[s * per + rh].x);
-  mm = wave_max_f32(mm);
-  const float base = mm == -__builtin_inff() ? 0.f : mm;
-  float acc[PL], l = 0.f;
-#pragma unroll
-  for (int j = 0; j < PL; ++j) acc[j] = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float2 ml = a.ml[s * per + rh];
-    const float w = exp2_hw(ml.x - base);
-    l = fmaf(w, ml.y, l);
-    const float* v = a.part + (s * per + rh) * D + PL * lane;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) acc[j] = fmaf(w, v[j], acc[j]);
+  constexpr int LR = D / 4, RW = kWave / LR, STEP = RW * WPH;  // lanes a range, ranges a wave, ranges a turn
+  __shared__ v4f_t racc[4][LR];
+  __shared__ float rl[4], rm[4];
+  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), part = wave % WPH, r = blockIdx.x, head = (int)blockIdx.y * (4 / WPH) + wave / WPH;
+  const Seq s0 = seq_of(a, lane);
+  const int chunk = own_plan(a, s0, lane).chunk;
+  // the row's sequence
+  Seq s{0, 0, 0, 0};
+  int before = 0, run = 0;
+  bool found = false;
+  for (int j0 = 0; j0 < a.b.B && !found; j0 += kWave) {
+    const Seq t = j0 ? seq_of(a, j0 + lane) : s0;
+    const int mine = t.tiles * ranges_of(t, chunk), upto = run + wave_scan(mine);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(t.rows > 0 && t.first <= r && r < t.first + t.rows);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      before = __builtin_amdgcn_readlane(upto - mine, l), found = true;
+      s = Seq{__builtin_amdgcn_readlane(t.first, l), __builtin_amdgcn_readlane(t.rows, l), __builtin_amdgcn_readlane(t.len, l), __builtin_amdgcn_readlane(t.tiles, l)};
+    }
+    run = __builtin_amdgcn_readlane(upto, 63);
   }
-  const float vs = a.c.fmt == DSGX_KV_E4M3 ? a.c.vs[head / a.G] : 1.f, inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
-  uint16_t* o = a.out + (size_t)r * a.ldo + (size_t)head * D + PL * lane;
+  const int own = ranges_of(s, chunk);
+  if (!found || (a.pre.splits == 0 && own == 1)) return;  // (the same for the whole workgroup)
+  const bool live = head < a.Hq;
+  const int h = (live ? head : 0) / a.G, px = r * a.G + head % a.G, ox = (r - s.first) * a.G + head % a.G;
+  const int n = live ? a.pre.splits + own : 0;
+  auto place_of = [&](int i) -> int64_t {
+    if (i < a.pre.splits) return (int64_t)((i * a.c.Hkv + h) * a.pre.tiles + px / a.pre.cols) * a.pre.cols + px % a.pre.cols;
+    const int item = (before + (i - a.pre.splits) * s.tiles + ox / a.own.cols) * a.c.Hkv + h;
+    return item < a.own.most ? own_places(a) + (int64_t)item * a.own.cols + ox % a.own.cols : -1;
+  };
+  const int sub = lane / LR, d = 4 * (lane % LR);
+  v4f_t acc = {0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+  constexpr int U = 4;  // ranges in flight a lane
+  for (int i0 = part * RW + sub; i0 < n; i0 += U * STEP) {
+    float2 ml[U];
+    v4f_t v[U];
 #pragma unroll
-  for (int j = 0; j < PL; ++j) o[j] = (uint16_t)f32_to_bf16_bits(acc[j] * inv);
-  if (lane == 0 && a.lse) a.lse[rh] = l == 0.f ? -__builtin_inff() : (mm + __builtin_amdgcn_logf(l)) * kLn2;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * STEP;
+      const int64_t at = i < n ? place_of(i) : -1;
+      ml[u] = at >= 0 ? a.ml[at] : make_float2(-__builtin_inff(), 0.f);
+      v[u] = at >= 0 ? *reinterpret_cast<const v4f_t*>(a.part + at * D + d) : v4f_t{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float to = fmaxf(m, ml[u].x), base = to == -__builtin_inff() ? 0.f : to, w0 = exp2_hw(m - base), w1 = exp2_hw(ml[u].x - base);
+      m = to, l = fmaf(l, w0, ml[u].y * w1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(acc[j], w0, v[u][j] * w1);
+    }
+  }
+  auto join = [&](float om, float ol, v4f_t ov) {
+    const float to = fmaxf(m, om), base = to == -__builtin_inff() ? 0.f : to, w0 = exp2_hw(m - base), w1 = exp2_hw(om - base);
+    m = to, l = fmaf(l, w0, ol * w1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = fmaf(acc[j], w0, ov[j] * w1);
+  };
+#pragma unroll
+  for (int k = LR; k < kWave; k <<= 1) {
+    v4f_t ov;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ov[j] = __shfl_xor(acc[j], k);
+    join(__shfl_xor(m, k), __shfl_xor(l, k), ov);
+  }
+  if (WPH > 1) {
+    if (sub == 0) racc[wave][lane] = acc;
+    if (lane == 0) rm[wave] = m, rl[wave] = l;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int k = 1; k < WPH; ++k) join(rm[wave + k], rl[wave + k], racc[wave + k][lane % LR]);
+  }
+  if (!live || sub) return;
+  const float vs = a.c.fmt == DSGX_KV_E4M3 ? a.c.vs[h] : 1.f, inv = l == 0.f ? 0.f : __fdiv_rn(vs, l);
+  *reinterpret_cast<uint2*>(a.out + (size_t)r * a.ldo + (size_t)head * D + d) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+  if (lane == 0 && a.lse) a.lse[(size_t)r * a.Hq + head] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 int round_up(int64_t v, int m) { return (int)((v + m - 1) / m * m); }
 
-// How a set of tokens is worked on by `cols` query columns: sixteen of them a workgroup, or tiles through LDS for 64 or 128
-enum Kind { kNarrow, kWide16, kWide32 };
-Kind kind_of(int64_t cols) {
-  return cols <= 16 ? kNarrow : cols <= 64 ? kWide16 : kWide32;
+// How `cols` query columns over the same tokens are worked on: 16 or 32 a workgroup from registers, 64 or 128 over tiles in LDS
+enum Kind { kNarrow16, kNarrow32, kWide64, kWide128 };
+Kind kind_of(int64_t cols, int D) { return cols <= 16 ? kNarrow16 : cols <= 32 && D < 256 ? kNarrow32 : cols <= 64 ? kWide64 : kWide128; }
+int cols_of(Kind k) { return 16 << k; }
+// workgroups a CU holds
+int resident(Kind k, int D, bool f8) {
+  if (k <= kNarrow32) return D == 64 ? 3 : D == 128 || f8 ? 2 : 1;
+  return D == 256 && k == kWide128 ? 1 : 2;
 }
-int cols_of(Kind k) { return k == kNarrow ? 16 : k == kWide16 ? 64 : 128; }
 
-Plan make_plan(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
-  const int G = Hq / c.Hkv, cus = num_cus_cached();
-  auto cut = [&](int64_t len, int64_t cols, int64_t sets, int& n, int& chunk) {
-    const Kind k = kind_of(cols);
-    const int64_t tiles = sets * c.Hkv * ((cols + cols_of(k) - 1) / cols_of(k));  // workgroups a range
-    const int64_t want = std::max<int64_t>(1, (k == kNarrow ? 4 : 2) * (int64_t)cus / std::max<int64_t>(1, tiles));
-    chunk = std::max(256, round_up((len + want - 1) / want, 128));
-    n = (int)std::max<int64_t>(1, (len + chunk - 1) / chunk);
-  };
-  Plan p{0, 128, 1, 128};
-  if (b.prefix_len) cut(b.prefix_len, (int64_t)b.rows * G, 1, p.sp, p.cp);
-  cut(b.max_len, (int64_t)b.max_rows * G, b.B, p.so, p.co);
-  return p;
+// Heads side by side a workgroup of the register kernels: their tokens' rows are neighbours in the usual layout of a page
+int heads_of(Kind k, const dsgx_kv_cache& c) {
+  return k > kNarrow32 || c.head_stride > c.tok_stride ? 1 : c.Hkv % 4 == 0 ? 4 : c.Hkv % 2 == 0 ? 2 : 1;
 }
-size_t ml_bytes(const Plan& p, const dsgx_kv_batch& b, int Hq) { return align256((size_t)(p.sp + p.so) * b.rows * Hq * sizeof(float2)); }
+
+struct Layout {
+  Kind kp, ko;
+  Part pre;
+  Own own;
+  int own_grid;
+  size_t ml, part;  // bytes
+};
+Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
+  const int G = Hq / c.Hkv, cus = num_cus_cached();
+  const bool f8 = c.fmt == DSGX_KV_E4M3;
+  Layout y{};
+  int64_t slots = 0;
+  if (b.prefix_len) {
+    const int64_t cols = (int64_t)b.rows * G;
+    y.kp = kind_of(cols, c.D);
+    y.pre.cols = cols_of(y.kp), y.pre.tiles = (int)((cols + y.pre.cols - 1) / y.pre.cols);
+    y.pre.heads = heads_of(y.kp, c);
+    const int64_t each = (int64_t)(c.Hkv / y.pre.heads) * y.pre.tiles, room = (int64_t)cus * resident(y.kp, c.D, f8);
+    y.pre.chunk = std::max(256, round_up((b.prefix_len + room / each) / std::max<int64_t>(1, room / each), 128));
+    y.pre.splits = (b.prefix_len + y.pre.chunk - 1) / y.pre.chunk;
+    slots = each * y.pre.heads * y.pre.splits * y.pre.cols;
+  }
+  y.ko = kind_of((int64_t)b.max_rows * G, c.D);
+  y.own.cols = cols_of(y.ko), y.own.heads = heads_of(y.ko, c);
+  const int room = cus * resident(y.ko, c.D, f8);
+  // short contexts without a prefix: a range a sequence, which leaves nothing to join
+  y.own.target = !b.prefix_len && b.max_len <= 512 ? 0 : room, y.own.least = 256;
+  const int64_t most = 4 * (int64_t)y.own.target * y.own.heads + (int64_t)c.Hkv * (((int64_t)b.rows * G) / y.own.cols + b.B + 1);
+  y.own.most = (int)std::min<int64_t>(most, 1 << 30);
+  y.own_grid = (int)std::min<int64_t>(room, most);
+  slots += (int64_t)y.own.most * y.own.cols;
+  y.ml = align256((size_t)slots * sizeof(float2)), y.part = align256((size_t)slots * c.D * 4);
+  return y;
+}
 
 template <int D, bool F8>
-int launch_part(const AttnArgs& a, int prefix, hipStream_t st) {
-  const int64_t cols = (int64_t)(prefix ? a.b.rows : a.b.max_rows) * a.G;
-  const Kind k = kind_of(cols);
-  const size_t lds = k == kNarrow ? (4 * 16 * (D + 4) + 128) * 4 : 4 * Wide<D, F8, 32>::kTile;
-  auto kern = k == kNarrow ? k_attn_narrow<D, F8> : k == kWide16 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
+int launch_part(const AttnArgs& a, Kind k, unsigned grid, int prefix, hipStream_t st) {
+  const int cols = cols_of(k);
+  const size_t lds = k <= kNarrow32 ? (size_t)(4 * cols * (D + 4) + 8 * cols) * 4 : 4 * Wide<D, F8, 32>::kTile;
+  auto kern = k == kNarrow16 ? k_attn_narrow<D, F8, 1> : k == kNarrow32 && D < 256 ? k_attn_narrow<(D < 256 ? D : 64), F8, 2> : k == kWide64 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
   if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
-  const dim3 grid((prefix ? a.p.sp : a.p.so) * a.c.Hkv, (unsigned)std::min<int64_t>(65535, (cols + cols_of(k) - 1) / cols_of(k)), prefix ? 1 : a.b.B);
-  hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a, prefix);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, st, a, prefix);
   DSGX_HIP(hipGetLastError());
   return DSGX_OK;
 }
 template <int D, bool F8>
-int launch(const AttnArgs& a, hipStream_t st) {
-  if (a.p.sp)
-    if (int rc = launch_part<D, F8>(a, 1, st)) return rc;
-  if (int rc = launch_part<D, F8>(a, 0, st)) return rc;
-  if (a.p.sp + a.p.so > 1) {
-    hipLaunchKernelGGL(k_combine<D>, dim3(a.b.rows, (a.Hq + 3) / 4), dim3(256), 0, st, a);
-    DSGX_HIP(hipGetLastError());
+int launch(const AttnArgs& a, const Layout& y, hipStream_t st) {
+  if (a.pre.splits) {
+    const int64_t pairs = (int64_t)a.pre.splits * (a.c.Hkv / a.pre.heads);
+    if (int rc = launch_part<D, F8>(a, y.kp, (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles), 1, st)) return rc;
   }
+  if (int rc = launch_part<D, F8>(a, y.ko, (unsigned)y.own_grid, 0, st)) return rc;
+  if (!a.pre.splits && !a.own.target) return DSGX_OK;
+  if ((int64_t)a.b.rows * a.Hq <= 1024) hipLaunchKernelGGL((k_combine<D, 4>), dim3(a.b.rows, a.Hq), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_combine<D, 1>), dim3(a.b.rows, (a.Hq + 3) / 4), dim3(256), 0, st, a);
+  DSGX_HIP(hipGetLastError());
   return DSGX_OK;
 }
 
@@ -781,8 +1056,8 @@ using namespace dsgx;
 
 extern "C" size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, int Hq) {
   if (check(cache, batch, Hq)) return 0;
-  const Plan p = make_plan(*cache, *batch, Hq);
-  return ml_bytes(p, *batch, Hq) + align256((size_t)(p.sp + p.so) * batch->rows * Hq * cache->D * 4) + 256;
+  const Layout y = make_layout(*cache, *batch, Hq);
+  return y.ml + y.part;
 }
 
 extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale, uint16_t* out, int64_t ldo,
@@ -795,16 +1070,17 @@ extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch,
     return fail(DSGX_EINVAL, "attn: rows %lld, %lld apart (multiples of 8, %lld at least; 16-byte aligned)", (long long)ldq, (long long)ldo, (long long)vals);
   if (batch->rows == 0) return DSGX_OK;
   AttnArgs a{};
-  a.c = *cache, a.b = *batch, a.p = make_plan(*cache, *batch, Hq);
+  const Layout y = make_layout(*cache, *batch, Hq);
+  a.c = *cache, a.b = *batch, a.pre = y.pre, a.own = y.own;
   a.q = q, a.out = out, a.lse = lse, a.ldq = ldq, a.ldo = ldo, a.Hq = Hq, a.G = Hq / cache->Hkv, a.page_shift = __builtin_ctz((unsigned)cache->page);
   a.scale2 = scale == 0.f ? 1.f : std::fabs(scale) * kLog2e, a.q_flip = scale < 0.f ? 0x80008000u : 0u, a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu;
   a.ml = static_cast<float2*>(ws);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ml_bytes(a.p, *batch, Hq));
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + y.ml);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f8 = cache->fmt == DSGX_KV_E4M3;
   switch (cache->D) {
-    case 64: return f8 ? launch<64, true>(a, st) : launch<64, false>(a, st);
-    case 128: return f8 ? launch<128, true>(a, st) : launch<128, false>(a, st);
-    default: return f8 ? launch<256, true>(a, st) : launch<256, false>(a, st);
+    case 64: return f8 ? launch<64, true>(a, y, st) : launch<64, false>(a, y, st);
+    case 128: return f8 ? launch<128, true>(a, y, st) : launch<128, false>(a, y, st);
+    default: return f8 ? launch<256, true>(a, y, st) : launch<256, false>(a, y, st);
   }
 }
