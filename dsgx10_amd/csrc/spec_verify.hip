@@ -2,35 +2,37 @@
 // numbers that lie next to borders (a cumulative sum over the vocabulary against a random threshold), so all sums and probabilities are
 // f64: with f32 exponentials about one draw in a hundred of a flat distribution over 10^5 tokens would come out one token off.
 //
-// Three launches: k_stats reads every row of logits once and leaves, for each chunk of it, the maximum, the sum of exp and the lowest
-// id of the maximum; k_weights judges its sequence's drafts (every workgroup for itself: a few KB out of L2), then sums the weights of
-// its chunk of the one row that the next token comes from; k_pick finds the chunk and the token in it. Probabilities need no k_stats.
+// Two launches: k_stats reads every row of logits once and leaves, for each chunk of it, the maximum, the sum of exp and the lowest
+// id of the maximum; k_weights judges its sequence's drafts (every workgroup for itself: a few KB out of L2), sums the weights of
+// its chunk of the one row that the next token comes from, and the last workgroup of a sequence draws. Probabilities need no k_stats.
 #include "abi_internal.h"
 #include "common.cuh"
 
 namespace dsgx {
 namespace {
 
-constexpr int kChunk = 4096, kThreads = 256, kPer = kChunk / kThreads;
+constexpr int kChunk = 4096, kThreads = 512, kWaves = kThreads / kWave, kPer = kChunk / kThreads;  // k_weights
+constexpr int kStatChunk = 4096, kStatThreads = 256, kStatWaves = kStatThreads / kWave, kStatPer = kStatChunk / kStatThreads;
 
 struct Stat {  // of one chunk of one row; also of a whole row
   double sum;  // sum of exp((x - max) / T); T <= 0: 1, or NaN if the chunk holds one
   float max;
   int arg;
 };
-struct Judged {  // of one sequence
-  double max, scale;  // the drawn-from row: p = exp((x - max) * 1/T) * scale
-  int end, last, arg, rows0;
+struct Judged {  // of one sequence: the row that its next token comes from
+  double scale;  // p = exp((x - max) / T) * scale
+  float max;
+  int end, last, arg;
 };
 struct Sums {
   double rest, p;  // of max(p - q, 0) and of p over a chunk
 };
 struct VerifyArgs {
   dsgx_verify_in in;
-  int nc;
-  Stat* stat;      // [rows][nc]
+  int ns, nc;      // chunks of k_stats, of k_weights
+  Stat* stat;      // [rows][ns]
   Sums* sums;      // [B][nc]
-  Judged* judged;  // [B]
+  int* count;      // [B]: chunks done
   int32_t *tokens, *accepted;
 };
 
@@ -70,52 +72,110 @@ __device__ __forceinline__ const void* row_of(const void* base, int64_t ld, int 
   return static_cast<const uint8_t*>(base) + (KIND == 1 ? 2 : 4) * (ld * (int64_t)r);
 }
 
-// e^y for y <= 0 (a NaN stays one): y = n ln 2 + r with |r| <= ln 2 / 2, the Taylor sum of e^r up to r^13 (the next term is below
-// 2^-57) and 2^n. Twenty instructions where the library's exp, which has to serve every argument, takes about fifty: the exponentials
-// of the logits are what this operator computes most of.
-__device__ __forceinline__ double exp_neg(double y) {
-  y = y < -800.0 ? -800.0 : y;  // (e^-800 is 0 in f64)
-  const double n = rint(y * 1.4426950408889634074);
-  double r = fma(n, -0x1.62e42fefa39efp-1, y);
-  r = fma(n, -0x1.abc9e3b39803fp-56, r);  // (what the double nearest ln 2 leaves of it)
-  double s = 1.0 / 6227020800.0;
-  s = fma(s, r, 1.0 / 479001600.0);
-  s = fma(s, r, 1.0 / 39916800.0);
-  s = fma(s, r, 1.0 / 3628800.0);
-  s = fma(s, r, 1.0 / 362880.0);
-  s = fma(s, r, 1.0 / 40320.0);
-  s = fma(s, r, 1.0 / 5040.0);
-  s = fma(s, r, 1.0 / 720.0);
-  s = fma(s, r, 1.0 / 120.0);
-  s = fma(s, r, 1.0 / 24.0);
-  s = fma(s, r, 1.0 / 6.0);
-  s = fma(s, r, 0.5);
-  s = fma(s, r, 1.0);
-  s = fma(s, r, 1.0);
-  return ldexp(s, (int)n);
+// exp((x - max) / T) of f32 values in f64, for x <= max; a NaN gives NaN, an x that lies 700 T or more below the maximum e^-700 (10^-304,
+// which no sum notices) or with ZERO 0. (x - max) / T = (n + k / 64) ln 2 + r, |r| <= ln 2 / 128, the whole number 64 n + k rounded by adding
+// 1.5 * 2^52: 2^(k / 64) out of a table in LDS, times the Taylor sum of e^r up to r^4 (the next term is below 2^-44 of it), times 2^n on
+// the exponent's bits. Twelve f64 instructions a value, which is what bounds k_stats (a wave's takes about eight clocks); with the
+// range ln 2 wide and terms up to r^11 there were eighteen, and 80 rows of 131072 logits took 15.9 us. The library's exp takes about fifty.
+__constant__ double kExp2[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
+struct Exp {
+  double it, itl, max;  // 1 / T, 64 log2 e / T
+  float lo;             // max - 700 T
+  const double* tab;    // kExp2 in LDS
+};
+__device__ __forceinline__ Exp exp_of(float max, float T, double it, const double* tab) {
+  return Exp{it, it * (64.0 * 1.4426950408889634074), (double)max, max - 700.f * T, tab};
+}
+template <bool ZERO>
+__device__ __forceinline__ double exp_at(const Exp& e, float x) {
+  const bool none = x <= e.lo;
+  const double y = (double)(none ? e.lo : x) - e.max, t = fma(y, e.itl, 0x1.8p52), r = fma(t - 0x1.8p52, -0x1.62e42fefa39efp-7, y * e.it);
+  const int N = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+  const double c = e.tab[N & 63];
+  const double s = fma(c, r * fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), c);
+  // s lies in [0.99, 2), n in [-1011, 0]
+  const uint64_t b = __builtin_bit_cast(uint64_t, s);
+  const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(N >> 6) << 20);
+  const uint64_t v = (uint64_t)hi << 32 | (uint32_t)b;
+  return __builtin_bit_cast(double, ZERO && none ? (uint64_t)0 : v);
 }
 
-__device__ __forceinline__ double shfl_f64(double v, int src) {
+// sums and maxima over a wave by DPP steps within the rows of sixteen lanes and half swaps, in every lane
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl((int)(uint32_t)b, src), hi = __shfl((int)(b >> 32), src);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  return __builtin_bit_cast(double, (uint64_t)dpp_mov<CTRL>((uint32_t)(b >> 32)) << 32 | dpp_mov<CTRL>((uint32_t)b));
 }
-__device__ __forceinline__ double wave_sum_f64(double v, int lane) {
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v += dpp_f64<0xB1>(v);
+  v += dpp_f64<0x4E>(v);
+  v += dpp_f64<0x141>(v);
+  v += dpp_f64<0x140>(v);
+  uint64_t b = __builtin_bit_cast(uint64_t, v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false), hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  v = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+  b = __builtin_bit_cast(uint64_t, v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false), hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+// inclusive sums over the lanes (shifts within the rows, the rows' last lanes handed on)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double scan_step_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v = scan_step_f64<0x111, 0xF>(v);
+  v = scan_step_f64<0x112, 0xF>(v);
+  v = scan_step_f64<0x114, 0xF>(v);
+  v = scan_step_f64<0x118, 0xF>(v);
+  v = scan_step_f64<0x142, 0xA>(v);
+  return scan_step_f64<0x143, 0xC>(v);
+}
+__device__ __forceinline__ double readlane_f64(double v, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l));
+}
+__device__ __forceinline__ double sum_waves(const double* red) {
+  double v = red[0];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += shfl_f64(v, lane ^ d);
+  for (int w = 1; w < kWaves; ++w) v += red[w];
   return v;
-}
-__device__ __forceinline__ double block_sum_f64(double v, double* red, int lane, int wave) {
-  v = wave_sum_f64(v, lane);
-  __syncthreads();
-  if (lane == 0) red[wave] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
 }
 // the larger maximum, of equals the lower id
 __device__ __forceinline__ void take_max(float& m, int& arg, float om, int oa) {
   const bool t = om > m || (om == m && oa < arg);
   m = t ? om : m, arg = t ? oa : arg;
+}
+__device__ __forceinline__ void wave_take_max(float& m, int& arg) {
+  take_max(m, arg, __uint_as_float(dpp_mov<0xB1>(__float_as_uint(m))), (int)dpp_mov<0xB1>((uint32_t)arg));
+  take_max(m, arg, __uint_as_float(dpp_mov<0x4E>(__float_as_uint(m))), (int)dpp_mov<0x4E>((uint32_t)arg));
+  take_max(m, arg, __uint_as_float(dpp_mov<0x141>(__float_as_uint(m))), (int)dpp_mov<0x141>((uint32_t)arg));
+  take_max(m, arg, __uint_as_float(dpp_mov<0x140>(__float_as_uint(m))), (int)dpp_mov<0x140>((uint32_t)arg));
+  auto f = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false), i = __builtin_amdgcn_permlane16_swap((uint32_t)arg, (uint32_t)arg, false, false);
+  m = __uint_as_float(f[0]), arg = (int)i[0];
+  take_max(m, arg, __uint_as_float(f[1]), (int)i[1]);
+  f = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false), i = __builtin_amdgcn_permlane32_swap((uint32_t)arg, (uint32_t)arg, false, false);
+  m = __uint_as_float(f[0]), arg = (int)i[0];
+  take_max(m, arg, __uint_as_float(f[1]), (int)i[1]);
 }
 
 // the sequence's rows; none if the bounds are out of order
@@ -135,248 +195,278 @@ __device__ __forceinline__ int seq_of(const dsgx_verify_in& in, int r, int lane)
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kThreads) k_stats(VerifyArgs a) {
-  constexpr int U = kUnit<KIND>, NU = kPer / U;
+__global__ void __launch_bounds__(kStatThreads) k_stats(VerifyArgs a) {
+  constexpr int U = kUnit<KIND>, NU = kStatPer / U;
   const dsgx_verify_in& in = a.in;
-  __shared__ double red[4];
-  __shared__ float rm[4];
-  __shared__ int ra[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y, c = blockIdx.x;
+  __shared__ double red[kStatWaves], tab[64];
+  __shared__ float rm[kStatWaves];
+  __shared__ int ra[kStatWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y, v0 = blockIdx.x * kStatChunk + (int)threadIdx.x * U;
+  const void* row = row_of<KIND>(in.target, in.ldt, r);
+  float x[NU][U];  // (on their way before anything is waited for)
+#pragma unroll
+  for (int k = 0; k < NU; ++k) load_unit<KIND>(row, v0 + k * kStatThreads * U, in.V, -__builtin_inff(), x[k]);
+  if (threadIdx.x < 64) tab[threadIdx.x] = kExp2[threadIdx.x];
   const int b = seq_of(in, r, lane);
   if (b < 0 || b >= in.B) return;
   const float T = in.temp ? in.temp[b] : 1.f;
-  const void* row = row_of<KIND>(in.target, in.ldt, r);
-  float x[NU][U];
-#pragma unroll
-  for (int k = 0; k < NU; ++k) load_unit<KIND>(row, c * kChunk + (k * kThreads + (int)threadIdx.x) * U, in.V, -__builtin_inff(), x[k]);
+  const bool greedy = !(T > 0.f || T != T);
   float m = -__builtin_inff();
   int arg = 0x7FFFFFFF;
 #pragma unroll
   for (int k = 0; k < NU; ++k)
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int v = c * kChunk + (k * kThreads + (int)threadIdx.x) * U + i;
-      if (x[k][i] > m) m = x[k][i], arg = v;  // (ids rise within a thread: the first of equals stays)
-    }
+    for (int i = 0; i < U; ++i) m = fmaxf(m, x[k][i]);
+  if (greedy) {  // (the id of the maximum is asked for nowhere else)
 #pragma unroll
-  for (int d = 32; d; d >>= 1) take_max(m, arg, __shfl_xor(m, d), __shfl_xor(arg, d));
+    for (int k = NU - 1; k >= 0; --k)
+#pragma unroll
+      for (int i = U - 1; i >= 0; --i) arg = x[k][i] == m && m != -__builtin_inff() ? v0 + k * kStatThreads * U + i : arg;
+    wave_take_max(m, arg);
+  } else {
+    m = wave_max_f32(m);
+  }
   if (lane == 0) rm[wave] = m, ra[wave] = arg;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) take_max(m, arg, rm[w], ra[w]);
+  for (int w = 0; w < kStatWaves; ++w) take_max(m, arg, rm[w], ra[w]);
   double s = 0.0;
-  if (T > 0.f || T != T) {
-    const double it = 1.0 / (double)T, md = m;
+  if (!greedy && m != -__builtin_inff()) {
+    const Exp e = exp_of(m, T, 1.0 / (double)T, tab);
 #pragma unroll
     for (int k = 0; k < NU; ++k)
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const float xv = x[k][i];
-        // (a chunk of nothing but -inf has no maximum to subtract)
-        s += m == -__builtin_inff() ? (xv == xv ? 0.0 : (double)xv) : exp_neg(((double)xv - md) * it);
-      }
-  } else {
+      for (int i = 0; i < U; ++i) s += exp_at<false>(e, x[k][i]);
+  } else {  // whether there is a NaN; a greedy row's sum is 1 (a chunk of nothing but -inf has no maximum to subtract, and the sum 0)
+    float f = 0.f;
 #pragma unroll
     for (int k = 0; k < NU; ++k)
 #pragma unroll
-      for (int i = 0; i < U; ++i) s += x[k][i] == x[k][i] ? 0.0 : (double)x[k][i];
-    if (threadIdx.x == 0) s += 1.0;
+      for (int i = 0; i < U; ++i) f = x[k][i] == x[k][i] ? f : x[k][i];
+    s = (double)f + (greedy && threadIdx.x == 0 ? 1.0 : 0.0);
   }
-  s = block_sum_f64(s, red, lane, wave);
-  if (threadIdx.x == 0) a.stat[(size_t)r * a.nc + c] = Stat{s, m, arg};
+  s = wave_sum_f64(s);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kStatWaves; ++w) s += red[w];
+    a.stat[(size_t)r * a.ns + blockIdx.x] = Stat{s, m, arg};
+  }
 }
 
-// A row's statistics out of its chunks', by one wave; wave-uniform
-__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, int r, float T, int lane) {
-  float m = -__builtin_inff();
-  int arg = 0x7FFFFFFF;
-  const Stat* st = a.stat + (size_t)r * a.nc;
-  for (int c = lane; c < a.nc; c += kWave) take_max(m, arg, st[c].max, st[c].arg);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) take_max(m, arg, __shfl_xor(m, d), __shfl_xor(arg, d));
-  double s = 0.0;
-  const double it = 1.0 / (double)T;
-  for (int c = lane; c < a.nc; c += kWave) {
-    const double cs = st[c].sum;
-    if (!(T > 0.f || T != T)) s += cs;
-    else s += cs == 0.0 ? 0.0 : cs * exp_neg(((double)st[c].max - (double)m) * it);
-  }
-  return Stat{wave_sum_f64(s, lane), m, arg};
+// A row's statistics out of its chunks' (the lane's own st, chunks lane, lane + 64, ..), by one wave
+__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, int r, float T, double it, const double* tab, int lane, Stat st) {
+  float m = st.max;
+  int arg = st.arg;
+  const Stat* more = a.stat + (size_t)r * a.ns;
+  for (int c = lane + kWave; c < a.ns; c += kWave) take_max(m, arg, more[c].max, more[c].arg);
+  wave_take_max(m, arg);
+  const bool greedy = !(T > 0.f || T != T);
+  const Exp e = exp_of(m, T, it, tab);
+  auto part = [&](const Stat& x) { return greedy ? x.sum : x.sum == 0.0 ? 0.0 : x.sum * exp_at<true>(e, x.max); };
+  double s = part(st);
+  for (int c = lane + kWave; c < a.ns; c += kWave) s += part(more[c]);
+  return Stat{wave_sum_f64(s), m, arg};
 }
 
 // p of a value: logits x, or the probability itself
 template <int KIND>
-__device__ __forceinline__ double prob(float x, int v, const Judged& j, double it, bool greedy) {
+__device__ __forceinline__ double prob(float x, int v, const Judged& j, const Exp& e, bool greedy) {
   if (KIND == 2) return (double)x;
   if (greedy) return v == j.arg ? j.scale : 0.0 * j.scale;  // (a row with a NaN has a NaN scale)
-  return exp_neg(((double)x - j.max) * it) * j.scale;
+  return exp_at<true>(e, x) * j.scale;
 }
 __device__ __forceinline__ double rest_of(double p, double q) {
   const double d = p - q;
-  return d > 0.0 ? d : d == d ? 0.0 : d;
+  const uint64_t b = __builtin_bit_cast(uint64_t, d);
+  return __builtin_bit_cast(double, d <= 0.0 ? (uint64_t)0 : b);  // (a NaN stays)
 }
 
-// the drafts of sequence b up to the first that is refused; by the whole workgroup
+// the drafts of sequence b up to the first that is refused, by the whole workgroup, a wave a row
 template <int KIND>
-__device__ __forceinline__ Judged judge(const VerifyArgs& a, int b, int r0, int r1, float T, int lane, int wave, Judged* sh, int* stop) {
+__device__ __forceinline__ Judged judge(const VerifyArgs& a, int r0, int r1, float T, double it, const double* tab, int lane, int wave, Judged* sh, int* stop) {
   const dsgx_verify_in& in = a.in;
   const bool greedy = !(T > 0.f || T != T);
-  const double it = 1.0 / (double)T;
-  for (int i0 = r0;; i0 += 4) {
+  for (int i0 = r0;; i0 += kWaves) {
     const int r = i0 + wave;
     bool stops = false;
-    Judged j{0.0, 1.0, r, 0, -1, r0};
+    Judged j{1.0, -__builtin_inff(), r, 0, -1};
     if (r < r1) {
+      // everything that can be asked for now: the chunks' statistics, the draft and its random number, then the draft's own values
+      Stat st{0.0, -__builtin_inff(), 0x7FFFFFFF};
+      if (KIND != 2 && lane < a.ns) st = a.stat[(size_t)r * a.ns + lane];
+      j.last = r == r1 - 1;
+      const int d = j.last ? -1 : in.draft[r];
+      const float u = j.last ? 0.f : in.u[r];
+      float x = 0.f;
+      double q = 1.0;
+      const bool known = d >= 0 && d < in.V;
+      if (known) {
+        const void* row = row_of<KIND>(in.target, in.ldt, r);
+        x = KIND == 1 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[d]) : static_cast<const float*>(row)[d];
+        if (in.q) q = in.q[in.ldq * (int64_t)r + d];
+      }
       if (KIND != 2) {
-        const Stat s = row_stat(a, r, T, lane);
+        const Stat s = row_stat(a, r, T, it, tab, lane, st);
         j.max = s.max, j.arg = s.arg;
         j.scale = greedy ? s.sum * 0.0 + 1.0 : 1.0 / s.sum;
       }
-      j.last = r == r1 - 1;
-      stops = j.last;
-      if (!j.last) {
-        const int d = in.draft[r];
-        double p = 0.0, q = 1.0;
-        if (d >= 0 && d < in.V) {
-          const void* row = row_of<KIND>(in.target, in.ldt, r);
-          const float x = KIND == 1 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[d]) : static_cast<const float*>(row)[d];
-          p = prob<KIND>(x, d, j, it, greedy);
-          if (in.q) q = in.q[in.ldq * (int64_t)r + d];
-        }
-        stops = !((double)in.u[r] * q < p);
-      }
+      const double p = known ? prob<KIND>(x, d, j, exp_of(j.max, T, it, tab), greedy) : 0.0;
+      stops = j.last || !((double)u * q < p);
     }
     __syncthreads();
     if (lane == 0) sh[wave] = j, stop[wave] = stops;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < kWaves; ++w)
       if (stop[w]) return sh[w];
   }
 }
 
 // the weights of U ids from v on of the judged row: rest = max(p - q, 0) (the last row: p), and p
 template <int KIND>
-__device__ __forceinline__ void weights(const VerifyArgs& a, const Judged& j, double it, bool greedy, int v, double (&rest)[kUnit<KIND>], double (&p)[kUnit<KIND>]) {
+__device__ __forceinline__ void weights(const VerifyArgs& a, const Judged& j, const Exp& e, bool greedy, int v, double (&rest)[kUnit<KIND>], double (&p)[kUnit<KIND>]) {
   constexpr int U = kUnit<KIND>;
   const dsgx_verify_in& in = a.in;
-  float x[U];
+  float x[U], q[U];
   load_unit<KIND>(row_of<KIND>(in.target, in.ldt, j.end), v, in.V, KIND == 2 ? 0.f : -__builtin_inff(), x);
-#pragma unroll
-  for (int i = 0; i < U; ++i) p[i] = v + i < in.V ? prob<KIND>(x[i], v + i, j, it, greedy) : 0.0;
-  if (j.last) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) rest[i] = p[i];
-  } else if (in.q) {
+  const bool drafter = !j.last && in.q;
+  if (drafter) {
     const float* qr = in.q + in.ldq * (int64_t)j.end;
 #pragma unroll
     for (int h = 0; h < U; h += 4) {
-      float q[4];
-      load_unit<0>(qr, v + h, in.V, 0.f, q);
+      float t[4];
+      load_unit<0>(qr, v + h, in.V, 0.f, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rest[h + i] = rest_of(p[h + i], (double)q[i]);
+      for (int i = 0; i < 4; ++i) q[h + i] = t[i];
     }
   } else {
-    const int d = in.draft[j.end];
+    const int d = j.last ? -1 : in.draft[j.end];
 #pragma unroll
-    for (int i = 0; i < U; ++i) rest[i] = rest_of(p[i], v + i == d ? 1.0 : 0.0);
+    for (int i = 0; i < U; ++i) q[i] = v + i == d ? 1.f : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    p[i] = v + i < in.V ? prob<KIND>(x[i], v + i, j, e, greedy) : 0.0;
+    rest[i] = j.last ? p[i] : rest_of(p[i], (double)q[i]);
   }
 }
 
+// values that another workgroup's thread wrote and this one may read without either side's cache in between
+__device__ __forceinline__ void put_f64(double* p, double v) {
+  __hip_atomic_store((DSGX_GLOBAL uint64_t*)(uintptr_t)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get_f64(const double* p) {
+  return __builtin_bit_cast(double, __hip_atomic_load((const DSGX_GLOBAL uint64_t*)(uintptr_t)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Judges its sequence's drafts and sums the weights of its chunk of the row that the next token comes from; the workgroup that is the
+// sequence's last to be done finds the chunk and the token in it. (The sums reach memory before the count does: they are
+// device-scope stores, and the count waits for their acknowledgement. The last one sets the count back for the next call.)
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) k_weights(VerifyArgs a) {
   constexpr int U = kUnit<KIND>, NU = kPer / U;
-  __shared__ double red[4];
-  __shared__ Judged sh[4];
-  __shared__ int stop[4];
+  __shared__ double red[2 * kWaves], tab[64];
+  __shared__ Judged sh[kWaves];
+  __shared__ int stop[kWaves], is_last, hits[kWaves], lasts[kWaves];
   const dsgx_verify_in& in = a.in;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.y, c = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y, c = blockIdx.x;
+  const float T = KIND != 2 && in.temp ? in.temp[b] : 1.f, us = in.us[b];
   int r0, r1;
-  if (!rows_of(in, b, r0, r1)) return;
-  const float T = KIND != 2 && in.temp ? in.temp[b] : 1.f;
+  if (!rows_of(in, b, r0, r1)) {
+    if (c == 0 && tid == 0) a.accepted[b] = 0;
+    return;
+  }
   const bool greedy = !(T > 0.f || T != T);
-  const Judged j = judge<KIND>(a, b, r0, r1, T, lane, wave, sh, stop);
   const double it = 1.0 / (double)T;
+  if (KIND != 2) {
+    if (tid < 64) tab[tid] = kExp2[tid];
+    __syncthreads();
+  }
+  const Judged j = judge<KIND>(a, r0, r1, T, it, tab, lane, wave, sh, stop);
+  const Exp e = exp_of(j.max, T, it, tab);
   double sr = 0.0, sp = 0.0;
 #pragma unroll
   for (int k = 0; k < NU; ++k) {
     double rest[U], p[U];
-    weights<KIND>(a, j, it, greedy, c * kChunk + (k * kThreads + (int)threadIdx.x) * U, rest, p);
+    weights<KIND>(a, j, e, greedy, c * kChunk + (k * kThreads + tid) * U, rest, p);
 #pragma unroll
     for (int i = 0; i < U; ++i) sr += rest[i], sp += p[i];
   }
-  sr = block_sum_f64(sr, red, lane, wave);
-  sp = block_sum_f64(sp, red, lane, wave);
-  if (threadIdx.x == 0) {
-    a.sums[(size_t)b * a.nc + c] = Sums{sr, sp};
-    if (c == 0) a.judged[b] = j;
+  sr = wave_sum_f64(sr), sp = wave_sum_f64(sp);
+  if (lane == 0) red[wave] = sr, red[kWaves + wave] = sp;
+  __syncthreads();
+  Sums* sums = a.sums + (size_t)b * a.nc;
+  if (tid == 0) {
+    put_f64(&sums[c].rest, sum_waves(red)), put_f64(&sums[c].p, sum_waves(red + kWaves));
+    __builtin_amdgcn_s_waitcnt(0);
+    const int before = __hip_atomic_fetch_add((DSGX_GLOBAL int*)(uintptr_t)(a.count + b), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = before == a.nc - 1;
+    if (is_last) __hip_atomic_store((DSGX_GLOBAL int*)(uintptr_t)(a.count + b), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-}
+  __syncthreads();
+  if (!is_last) return;
 
-template <int KIND>
-__global__ void __launch_bounds__(kThreads) k_pick(VerifyArgs a) {
-  constexpr int U = kUnit<KIND>, NU = kPer / U;
-  __shared__ double part[kThreads];
-  __shared__ int hit, lastpos;
-  const dsgx_verify_in& in = a.in;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  int r0, r1;
-  if (!rows_of(in, b, r0, r1)) {
-    if (tid == 0) a.accepted[b] = 0;
-    return;
-  }
-  const Judged j = a.judged[b];
-  const float T = KIND != 2 && in.temp ? in.temp[b] : 1.f;
-  const bool greedy = !(T > 0.f || T != T);
-  const double it = 1.0 / (double)T;
-  const Sums* s = a.sums + (size_t)b * a.nc;
-  // the chunk sums in order, by every thread alike (tens of values out of L2)
-  double total = 0.0;
-  for (int c = 0; c < a.nc; ++c) total += s[c].rest;
+  // every wave alike: the chunks' sums, 64 at a time; the chunk is the first whose running sum passes the threshold
+  auto sum_of = [&](int i, bool of_p) { return i < a.nc ? get_f64(of_p ? &sums[i].p : &sums[i].rest) : 0.0; };
+  const double rest0 = sum_of(lane, false), p0 = sum_of(lane, true);
+  auto total_of = [&](bool of_p) {
+    double t = of_p ? p0 : rest0;
+    for (int i = lane + kWave; i < a.nc; i += kWave) t += sum_of(i, of_p);
+    return wave_sum_f64(t);
+  };
+  double total = total_of(false);
   const bool of_p = total <= 0.0;  // nothing left of the difference: from p
-  if (of_p) {
-    total = 0.0;
-    for (int c = 0; c < a.nc; ++c) total += s[c].p;
-  }
-  const double t = (double)in.us[b] * total;
+  if (of_p) total = total_of(true);
+  const double t = (double)us * total;
   int token = -1;
   if (total > 0.0 && total < __builtin_inf()) {
     double run = 0.0, before = 0.0;
     int chunk = 0;
-    for (int c = 0; c < a.nc; ++c) {
-      const double w = of_p ? s[c].p : s[c].rest;
-      if (w > 0.0) chunk = c, before = run;
-      run += w;
-      if (w > 0.0 && run > t) break;
+    for (int c0 = 0; c0 < a.nc; c0 += kWave) {
+      const double w = c0 ? sum_of(c0 + lane, of_p) : of_p ? p0 : rest0, upto = run + wave_scan_f64(w);
+      const uint64_t some = __builtin_amdgcn_ballot_w64(w > 0.0), past = __builtin_amdgcn_ballot_w64(w > 0.0 && upto > t);
+      if (some) {
+        const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // (none passes: rounding; the last that has any)
+        chunk = c0 + l, before = readlane_f64(upto, l) - readlane_f64(w, l);
+      }
+      if (past) break;
+      run = readlane_f64(upto, 63);
     }
-    // inside it: sixteen ids a thread, the threads' sums before a thread added in order
+    // inside it: eight ids a thread, and what stands before a thread's in order
     const int v0 = chunk * kChunk + tid * kPer;
     double w[kPer], mine = 0.0;
 #pragma unroll
     for (int k = 0; k < NU; ++k) {
       double rest[U], p[U];
-      weights<KIND>(a, j, it, greedy, v0 + k * U, rest, p);
+      weights<KIND>(a, j, e, greedy, v0 + k * U, rest, p);
 #pragma unroll
       for (int i = 0; i < U; ++i) w[k * U + i] = of_p ? p[i] : rest[i], mine += w[k * U + i];
     }
-    part[tid] = mine;
-    if (tid == 0) hit = 0x7FFFFFFF, lastpos = -1;
+    const double upto = wave_scan_f64(mine);
+    __syncthreads();  // (the sums in red have been read)
+    if (lane == 63) red[wave] = upto;
     __syncthreads();
-    double acc = before;
-    for (int k = 0; k < tid; ++k) acc += part[k];
+    double acc = before + (upto - mine);
+    for (int k = 0; k < wave; ++k) acc += red[k];
     int first = 0x7FFFFFFF, lastw = -1;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       acc += w[i];
-      if (w[i] > 0.0) {
-        lastw = v0 + i;
-        if (acc > t && first == 0x7FFFFFFF) first = v0 + i;
-      }
+      const bool any = w[i] > 0.0;
+      lastw = any ? v0 + i : lastw;
+      first = any && acc > t && first == 0x7FFFFFFF ? v0 + i : first;
     }
-    if (first != 0x7FFFFFFF) atomicMin(&hit, first);
-    if (lastw >= 0) atomicMax(&lastpos, lastw);
+    // ids rise with the lane and the wave: the first lane that passes the threshold, the last that has a weight
+    const uint64_t past = __builtin_amdgcn_ballot_w64(first != 0x7FFFFFFF), some = __builtin_amdgcn_ballot_w64(lastw >= 0);
+    const int wave_first = past ? __builtin_amdgcn_readlane(first, __builtin_ctzll(past)) : 0x7FFFFFFF, wave_last = some ? __builtin_amdgcn_readlane(lastw, 63 - __builtin_clzll(some)) : -1;
+    if (lane == 0) hits[wave] = wave_first, lasts[wave] = wave_last;
     __syncthreads();
-    token = hit != 0x7FFFFFFF ? hit : lastpos;  // (the sums' rounding can leave the threshold just past the chunk's end)
+    int hit = 0x7FFFFFFF, last = -1;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) hit = min(hit, hits[k]), last = max(last, lasts[k]);
+    token = hit != 0x7FFFFFFF ? hit : last;  // (the sums' rounding can leave the threshold just past the chunk's end)
   }
   for (int r = r0 + tid; r < r1; r += kThreads) a.tokens[r] = r < j.end ? in.draft[r] : r == j.end ? token : -1;
   if (tid == 0) a.accepted[b] = j.end - r0;
@@ -385,18 +475,17 @@ __global__ void __launch_bounds__(kThreads) k_pick(VerifyArgs a) {
 template <int KIND>
 int launch(const VerifyArgs& a, hipStream_t st) {
   if (KIND != 2) {
-    hipLaunchKernelGGL(k_stats<KIND>, dim3(a.nc, a.in.rows), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(k_stats<KIND>, dim3(a.ns, a.in.rows), dim3(kStatThreads), 0, st, a);
     DSGX_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL(k_weights<KIND>, dim3(a.nc, a.in.B), dim3(kThreads), 0, st, a);
-  DSGX_HIP(hipGetLastError());
-  hipLaunchKernelGGL(k_pick<KIND>, dim3(a.in.B), dim3(kThreads), 0, st, a);
   DSGX_HIP(hipGetLastError());
   return DSGX_OK;
 }
 
 bool sizes_ok(int B, int rows, int V) { return B >= 1 && B <= 65535 && rows >= 0 && rows <= 65535 && V >= 1 && V <= (1 << 28); }
-size_t stat_bytes(int rows, int nc) { return align256((size_t)rows * nc * sizeof(Stat)); }
+constexpr size_t kCountBytes = 65536 * sizeof(int);  // first in the workspace whatever the sizes: what a call leaves there is the next one's start
+size_t stat_bytes(int rows, int ns) { return align256((size_t)rows * ns * sizeof(Stat)); }
 size_t sums_bytes(int B, int nc) { return align256((size_t)B * nc * sizeof(Sums)); }
 
 }  // namespace
@@ -406,8 +495,7 @@ using namespace dsgx;
 
 extern "C" size_t dsgx_spec_verify_ws_bytes(int B, int rows, int V) {
   if (!sizes_ok(B, rows, V)) return 0;
-  const int nc = (V + kChunk - 1) / kChunk;
-  return stat_bytes(rows, nc) + sums_bytes(B, nc) + align256((size_t)B * sizeof(Judged));
+  return kCountBytes + stat_bytes(rows, (V + kStatChunk - 1) / kStatChunk) + sums_bytes(B, (V + kChunk - 1) / kChunk);
 }
 
 extern "C" int dsgx_spec_verify(const dsgx_verify_in* in, int32_t* tokens, int32_t* accepted, void* ws, void* stream) {
@@ -421,11 +509,11 @@ extern "C" int dsgx_spec_verify(const dsgx_verify_in* in, int32_t* tokens, int32
   if (((uintptr_t)ws & 15) || ((uintptr_t)in->target & (in->kind == 1 ? 1 : 3)) || ((uintptr_t)in->q & 3))
     return fail(DSGX_EINVAL, "spec_verify: workspace, target or probabilities not aligned");
   if (in->rows == 0) return DSGX_OK;
-  VerifyArgs a{*in, (in->V + kChunk - 1) / kChunk, nullptr, nullptr, nullptr, tokens, accepted};
+  VerifyArgs a{*in, (in->V + kStatChunk - 1) / kStatChunk, (in->V + kChunk - 1) / kChunk, nullptr, nullptr, nullptr, tokens, accepted};
   uint8_t* w = static_cast<uint8_t*>(ws);
-  a.stat = reinterpret_cast<Stat*>(w);
-  a.sums = reinterpret_cast<Sums*>(w + stat_bytes(in->rows, a.nc));
-  a.judged = reinterpret_cast<Judged*>(w + stat_bytes(in->rows, a.nc) + sums_bytes(in->B, a.nc));
+  a.count = reinterpret_cast<int*>(w);
+  a.stat = reinterpret_cast<Stat*>(w + kCountBytes);
+  a.sums = reinterpret_cast<Sums*>(w + kCountBytes + stat_bytes(in->rows, a.ns));
   hipStream_t st = static_cast<hipStream_t>(stream);
   return in->kind == 0 ? launch<0>(a, st) : in->kind == 1 ? launch<1>(a, st) : launch<2>(a, st);
 }
