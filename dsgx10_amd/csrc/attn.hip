@@ -567,13 +567,17 @@ __global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(
 // QW 32: v_mfma_f32_32x32x16_bf16, 128 columns a workgroup; QW 16: v_mfma_f32_16x16x32_bf16, 64 columns.
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 
+// a barrier for what passes through LDS alone: loads from memory stay on their way
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <int D, bool F8, int QW>
 struct Wide {
   static constexpr int KV = 8192 / D;            // tokens a tile
   static constexpr int SR = QW / 16 * 4 * (QW / 16);  // accumulators of a tile a lane: 16 or 4
   static constexpr int LG = kWave / QW;          // lanes that share a column: 2 or 4
   static constexpr int KD = 8 * LG;              // k of one instruction: 16 or 32
-  static constexpr int NS = D / KD, ST = KV / QW, OT = D / QW, NE = KV * QW / kWave, NP = NE / 8;
+  static constexpr int NS = D / KD, OT = D / QW;
+  static constexpr int NSUB = KV / 32, TS = 32 / QW, NE = QW / 2, NP = NE / 8;  // thirty-twos of a tile; score tiles, scores a lane, products' steps of one
   static constexpr int KN = F8 ? 2 : 4, VW = F8 ? 2 : 4;
   static constexpr int kTile = 16384;            // bytes of a tile of K, of V
   using acc_t = typename std::conditional<QW == 32, v16f_t, v4f_t>::type;
@@ -615,18 +619,25 @@ struct Wide {
   __device__ __forceinline__ static uint32_t v_group(uint32_t tid) { return tid / (D / 8); }  // of four tokens
 
   // at: byte offsets of the tile's sixteens (lane s % 16 .. of `offs`), from the head's first value
-  __device__ __forceinline__ static void load(Stage& x, const uint8_t* kh, const uint8_t* vh, uint64_t offs, uint32_t ts, uint32_t tid) {
-    auto off = [&](uint32_t sixteen) {
-      const uint32_t lo = __shfl((int)(uint32_t)offs, (int)sixteen), hi = __shfl((int)(offs >> 32), (int)sixteen);
+  __device__ __forceinline__ static void load(Stage& x, const uint8_t* kh, const uint8_t* vh, uint64_t offs, uint32_t ts, uint32_t tid, int wave) {
+    // (a wave's rows of a load lie in one sixteen: its place is wave-uniform, but for V with D 64)
+    auto off = [&](int sixteen) {
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)offs, sixteen), hi = __builtin_amdgcn_readlane((int)(offs >> 32), sixteen);
       return (uint64_t)hi << 32 | lo;
     };
 #pragma unroll
     for (int i = 0; i < KN; ++i) {
       const uint32_t row = k_row(i, tid);
-      x.k[i] = *(const DSGX_GLOBAL u32x4_t*)(uintptr_t)(kh + off(row / 16) + (row % 16) * ts + 16 * k_chunk(i, tid));
+      x.k[i] = *(const DSGX_GLOBAL u32x4_t*)((const DSGX_GLOBAL uint8_t*)(uintptr_t)(kh + off((int)k_row(i, 64 * wave) / 16)) + ((row % 16) * ts + 16 * k_chunk(i, tid)));
     }
     const uint32_t grp = v_group(tid), dc = tid % (D / 8);
-    const uint8_t* vb = vh + off(grp / 4) + (grp % 4) * 4 * ts + dc * VW * 4;
+    const uint8_t* vb;
+    if (D == 64) {
+      const uint32_t o0 = __shfl((int)(uint32_t)offs, (int)(grp / 4)), o1 = __shfl((int)(offs >> 32), (int)(grp / 4));
+      vb = vh + ((uint64_t)o1 << 32 | o0) + ((grp % 4) * 4 * ts + dc * VW * 4);
+    } else {
+      vb = vh + off((int)v_group(64 * wave) / 4) + ((grp % 4) * 4 * ts + dc * VW * 4);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (F8) {
@@ -695,7 +706,7 @@ template <int D, bool F8, int QW>
 __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide(AttnArgs a, int prefix) {
   using W = Wide<D, F8, QW>;
   using acc_t = typename W::acc_t;
-  constexpr int KV = W::KV, COLS = 4 * QW, NE = W::NE;
+  constexpr int KV = W::KV, COLS = 4 * QW;
   extern __shared__ __align__(16) uint8_t tiles[];  // two tiles of K and V each
   __shared__ int any_odd;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
@@ -739,13 +750,10 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
     float m = -__builtin_inff(), l = 0.f;  // m: the base, in scores; l: this lane's part of the sum
 
     // lane s < KV / 16: the page of the sixteen s of a tile, and where it lies
-    auto page_of = [&](int t0) {
-      const int t = t0 + 16 * (int)lane;
-      return (int)lane < KV / 16 && t < stop ? tab[t >> a.page_shift] : -1;
-    };
+    auto page_of = [&](int t0) { return tab[min(t0 + 16 * (int)lane, stop - 1) >> a.page_shift]; };  // (asked for with stop > 0 alone)
     auto place = [&](int t0, int page, uint32_t& there) {
       const int t = t0 + 16 * (int)lane;
-      const bool ok = page >= 0 && page < a.c.npages;
+      const bool ok = (int)lane < KV / 16 && t < stop && page >= 0 && page < a.c.npages;
       there = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
       return ok ? (uint64_t)(((int64_t)page * a.c.page_stride + (int64_t)(t & (a.c.page - 1)) * a.c.tok_stride) * esz) : 0ull;
     };
@@ -763,81 +771,123 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
       }
     };
 
+    // Thirty-two tokens at a time: while the matrix unit makes the next ones' scores, the vector unit makes these ones' numerators. A tile's
+    // successor is stored in its second half of LDS after everyone is done with the tile before (the turn's first barrier) and read
+    // after the second; the successor's successor is on its way in registers.
+    const uint32_t k_at = W::k_addr(col, lg), v_at = W::v_addr(col, lg);
+    auto scores = [&](const uint8_t* kt, uint32_t ka, int j, float (&e)[W::NE]) {
+      acc_t s[W::TS];
+#pragma unroll
+      for (int u = 0; u < W::TS; ++u)
+#pragma unroll
+        for (int i = 0; i < W::SR; ++i) s[u][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < W::NS; ++k)
+#pragma unroll
+        for (int u = 0; u < W::TS; ++u)
+          s[u] = W::mfma(__builtin_bit_cast(v8bf_t, *reinterpret_cast<const u32x4_t*>(kt + W::k_read(ka, W::TS * j + u, k))), q[k], s[u]);
+#pragma unroll
+      for (int u = 0; u < W::TS; ++u)
+#pragma unroll
+        for (int i = 0; i < W::SR; ++i) e[u * W::SR + i] = s[u][i];
+    };
+    auto fetch = [&](typename W::Stage& st, int t0, int page, uint32_t& there) {
+      const uint64_t at = place(t0, page, there);
+      W::load(st, kh, vh, at, ts, tid, wave);
+    };
     typename W::Stage st;
-    uint32_t there = 0, next_there = 0;
-    int page = page_of(lo), ahead = page_of(lo + KV);
-    __syncthreads();  // (the tiles of a column tile before this one have been read)
+    uint32_t there = 0, there1 = 0, there2 = 0;  // of the tile, the next, the one after
+    float e[W::NE];
+    lds_barrier();  // (the tiles of an item before this one have been read)
     if (lo < stop) {
-      const uint64_t at = place(lo, page, there);
-      W::load(st, kh, vh, at, ts, tid);
+      int ahead = page_of(lo + KV);
+      fetch(st, lo, page_of(lo), there);
       if (there != kAll || lo + KV > lim_lo) clean(st, lo, there);
       W::store(st, tiles, tiles + W::kTile, tid);
-    }
-    const uint32_t k_at = W::k_addr(col, lg), v_at = W::v_addr(col, lg);
-    int buf = 0;
-    for (int t0 = lo; t0 < stop; t0 += KV, buf ^= 1) {
-      __syncthreads();
-      const bool more = t0 + KV < stop;
-      if (more) {
-        const uint64_t at = place(t0 + KV, ahead, next_there);
-        W::load(st, kh, vh, at, ts, tid);
-        ahead = page_of(t0 + 2 * KV);
-      }
-      const uint8_t *kt = tiles + buf * 2 * W::kTile, *vt = kt + W::kTile;
-      uint32_t ka = k_at, va = v_at;
-      asm volatile("" : "+v"(ka), "+v"(va));  // (else every operand's address is kept in a register of its own)
-      float e[NE];
-#pragma unroll
-      for (int u = 0; u < W::ST; ++u) {
-        acc_t s;
-#pragma unroll
-        for (int j = 0; j < W::SR; ++j) s[j] = 0.f;
-#pragma unroll
-        for (int k = 0; k < W::NS; ++k)
-          s = W::mfma(__builtin_bit_cast(v8bf_t, *reinterpret_cast<const u32x4_t*>(kt + W::k_read(ka, u, k))), q[k], s);
-#pragma unroll
-        for (int j = 0; j < W::SR; ++j) e[u * W::SR + j] = s[j];
-      }
-      const bool all = there == kAll && t0 + KV <= lim_lo;
-      if (!all) {
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          const int tk = W::token_of(i, lg);
-          if (!(there >> (tk / 16) & 1) || t0 + tk >= lim) e[i] = -__builtin_inff();
-        }
-      }
-      float mx = e[0];
-#pragma unroll
-      for (int i = 1; i < NE; ++i) mx = fmaxf(mx, e[i]);
-      mx = __fmul_rn(column_max<QW>(mx), s2);
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {  // (-inf + slack: the first scores move it)
-        const float to = fmaxf(m, mx), base = to == -__builtin_inff() ? 0.f : to, alpha = exp2_hw(m - base);
-        l *= alpha, m = to;
-#pragma unroll
-        for (int i = 0; i < W::OT; ++i)
-#pragma unroll
-          for (int j = 0; j < W::SR; ++j) o[i][j] *= alpha;
-      }
-      const float base = m == -__builtin_inff() ? 0.f : m;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < NE; ++i) e[i] = exp2_hw(fmaf(e[i], s2, -base)), sum += e[i];
-      l += sum;
-      v8bf_t p[W::NP];
-#pragma unroll
-      for (int k = 0; k < W::NP; ++k) {
-        const u32x4_t pw = {pack_bf16(e[8 * k], e[8 * k + 1]), pack_bf16(e[8 * k + 2], e[8 * k + 3]), pack_bf16(e[8 * k + 4], e[8 * k + 5]), pack_bf16(e[8 * k + 6], e[8 * k + 7])};
-        p[k] = __builtin_bit_cast(v8bf_t, pw);
-      }
-#pragma unroll
-      for (int k = 0; k < W::NP; ++k)
-#pragma unroll
-        for (int i = 0; i < W::OT; ++i) o[i] = W::mfma(__builtin_bit_cast(v8bf_t, *reinterpret_cast<const u32x4_t*>(vt + W::v_read(va, i, k))), p[k], o[i]);
-      if (more) {
-        if (next_there != kAll || t0 + 2 * KV > lim_lo) clean(st, t0 + KV, next_there);
+      fetch(st, lo + KV, ahead, there1);
+      ahead = page_of(lo + 2 * KV);
+      lds_barrier();
+      scores(tiles, k_at, 0, e);
+      int buf = 0;
+      for (int t0 = lo; t0 < stop; t0 += KV, buf ^= 1) {
+        const uint8_t *kt = tiles + buf * 2 * W::kTile, *vt = kt + W::kTile;
         uint8_t* nt = tiles + (buf ^ 1) * 2 * W::kTile;
-        W::store(st, nt, nt + W::kTile, tid);
-        there = next_there;
+        uint32_t ka = k_at, va = v_at;
+        asm volatile("" : "+v"(ka), "+v"(va));  // (else every operand's address is kept in a register of its own)
+        if (there1 != kAll || t0 + 2 * KV > lim_lo) clean(st, t0 + KV, there1);
+        const bool all = there == kAll && t0 + KV <= lim_lo;
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < W::NSUB; ++j) {
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < W::NE; ++i) {
+              const int tk = 32 * j + W::token_of(i, lg);
+              if (!(there >> (tk / 16) & 1) || t0 + tk >= lim) e[i] = -__builtin_inff();
+            }
+          }
+          float mx = e[0];
+#pragma unroll
+          for (int i = 1; i < W::NE; ++i) mx = fmaxf(mx, e[i]);
+          mx = __fmul_rn(column_max<QW>(mx), s2);
+          if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {  // (-inf + slack: the first scores move it)
+            const float to = fmaxf(m, mx), base = to == -__builtin_inff() ? 0.f : to, alpha = exp2_hw(m - base);
+            l *= alpha, m = to;
+#pragma unroll
+            for (int i = 0; i < W::OT; ++i)
+#pragma unroll
+              for (int k = 0; k < W::SR; ++k) o[i][k] *= alpha;
+          }
+          const float base = m == -__builtin_inff() ? 0.f : m;
+          if (j == 0) {
+            W::store(st, nt, nt + W::kTile, tid);
+            fetch(st, t0 + 2 * KV, ahead, there2);  // (past the end: a tile of page 0, which is not looked at)
+            ahead = page_of(t0 + 3 * KV);
+          }
+          // The products of the next thirty-two's scores (M1), then of these numerators with V (M2), each with its share of the vector unit's
+          // work beside it, the operands read from LDS four products ahead. (sched_barrier: left to itself the compiler reads an operand
+          // right before its product, and every product waits for LDS.)
+          constexpr int M1 = W::NS * W::TS, M2 = W::NP * W::OT, PAIRS = W::NE / 2;
+          if (j == W::NSUB - 1) lds_barrier();
+          const uint8_t* kn = j < W::NSUB - 1 ? kt : nt;
+          auto operand = [&](int i) {
+            return i < M1 ? *reinterpret_cast<const u32x4_t*>(kn + W::k_read(ka, (j < W::NSUB - 1 ? W::TS * (j + 1) : 0) + i % W::TS, i / W::TS))
+                          : *reinterpret_cast<const u32x4_t*>(vt + W::v_read(va, (i - M1) % W::OT, W::NP * j + (i - M1) / W::OT));
+          };
+          u32x4_t ring[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ring[i] = operand(i);
+          acc_t s[W::TS];
+#pragma unroll
+          for (int u = 0; u < W::TS; ++u)
+#pragma unroll
+            for (int i = 0; i < W::SR; ++i) s[u][i] = 0.f;
+          uint32_t pw[PAIRS];
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < M1 + M2; ++i) {
+            if (i < M1) s[i % W::TS] = W::mfma(__builtin_bit_cast(v8bf_t, ring[i % 4]), q[i / W::TS], s[i % W::TS]);
+            else {
+              const int k = (i - M1) / W::OT, ot = (i - M1) % W::OT;
+              o[ot] = W::mfma(__builtin_bit_cast(v8bf_t, ring[i % 4]), __builtin_bit_cast(v8bf_t, u32x4_t{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]}), o[ot]);
+            }
+            if (i + 4 < M1 + M2) ring[i % 4] = operand(i + 4);
+            if (i < M1) {
+#pragma unroll
+              for (int w = i * PAIRS / M1; w < (i + 1) * PAIRS / M1; ++w) {
+                const float p0 = exp2_hw(fmaf(e[2 * w], s2, -base)), p1 = exp2_hw(fmaf(e[2 * w + 1], s2, -base));
+                l += p0, l += p1;
+                pw[w] = pack_bf16(p0, p1);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int u = 0; u < W::TS; ++u)
+#pragma unroll
+            for (int i = 0; i < W::SR; ++i) e[u * W::SR + i] = s[u][i];
+        }
+        there = there1, there1 = there2;
       }
     }
 
