@@ -38,6 +38,7 @@ struct AttnArgs {
   uint16_t* out;
   float *lse, *part;  // part: [places][cols][D], the prefix's first
   float2* ml;         // [places][cols]
+  int32_t* plan;      // [4 + B]: tokens a range, heads a workgroup; from 4 on every sequence's first item
   int64_t ldq, ldo;
   int Hq, G, page_shift;
   float scale2;              // |scale| log2 e; 1 for a scale of zero
@@ -72,7 +73,7 @@ __device__ __forceinline__ int wave_scan(int v) {
   v = scan_step<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3
   return scan_step<0x143, 0xC>(v);  // row_bcast 31 into rows 2 and 3
 }
-__device__ __forceinline__ int ranges_of(const Seq& s, int chunk) { return s.len ? (s.len + chunk - 1) / chunk : 1; }
+__device__ __forceinline__ int ranges_of(int len, int chunk) { return len ? (len + chunk - 1) / chunk : 1; }
 // Tokens a range of the sequences' own, by a whole wave; s: the lane's sequence of the first 64. The kernels that ask get the same answer.
 // A workgroup does a whole number of ranges one after the other: for one to four of them, ranges just long enough that there are no more of
 // them (each sequence's last one is short) than workgroups times that, and of the four the choice that is done first, a range's own
@@ -82,14 +83,28 @@ constexpr int kRangeCost = 192, kTogether = 96;
 struct Cut {
   int chunk, heads;
 };
-__device__ __forceinline__ Cut own_plan(const AttnArgs& a, const Seq& s, int lane) {
+__device__ __forceinline__ Cut own_plan(const AttnArgs& a, const Seq& s0, int lane) {
   if (a.own.target == 0) return Cut{1 << 30, 1};  // a range a sequence
-  float w = (float)s.tiles * (float)s.len;
-  for (int j0 = kWave; j0 < a.b.B; j0 += kWave) {
-    const Seq t = seq_of(a, j0 + lane);
-    w += (float)t.tiles * (float)t.len;
+  constexpr int KEPT = 4;  // sixty-fours of sequences in registers; the rest are read again every time
+  int tiles[KEPT], len[KEPT];
+#pragma unroll
+  for (int k = 0; k < KEPT; ++k) {
+    Seq t = s0;
+    if (k) t = k * kWave < a.b.B ? seq_of(a, k * kWave + lane) : Seq{0, 0, 0, 0};
+    tiles[k] = t.tiles, len[k] = t.len;
   }
-  w = uni(wave_sum(w)) * (float)a.c.Hkv * 1.0001f;
+  auto sum = [&](auto&& f) {
+    float v = f(tiles[0], len[0]);
+#pragma unroll
+    for (int k = 1; k < KEPT; ++k)
+      if (k * kWave < a.b.B) v += f(tiles[k], len[k]);
+    for (int j0 = KEPT * kWave; j0 < a.b.B; j0 += kWave) {
+      const Seq t = seq_of(a, j0 + lane);
+      v += f(t.tiles, t.len);
+    }
+    return uni(wave_sum(v));
+  };
+  float w = sum([](int t, int n) { return (float)t * (float)n; }) * (float)a.c.Hkv * 1.0001f;
   int heads = a.own.heads, best = 0;
   while (heads > 1 && w < (float)a.own.target * (float)(kTogether * heads)) heads >>= 1;
   const float groups = (float)(a.c.Hkv / heads);
@@ -97,31 +112,56 @@ __device__ __forceinline__ Cut own_plan(const AttnArgs& a, const Seq& s, int lan
   float cost = 3e38f;
 #pragma unroll 1
   for (int turns = 1; turns <= 4; ++turns) {
-    const float room = (float)(a.own.target * turns);
-    int chunk = max(heads > 1 ? 128 : a.own.least, ((int)min(w / room, 1e9f) + 128) & ~127);
+    const float room = (float)(a.own.target * turns), share = w / room;
+    if (share + (float)kRangeCost > cost / (float)turns) break;  // (not even without a loss)
+    int chunk = max(heads > 1 ? 128 : a.own.least, ((int)min(share, 1e9f) + 128) & ~127);
     float all = 0.f;
 #pragma unroll 1
     for (int k = 0; k < 3; ++k) {
-      int n = s.tiles * ranges_of(s, chunk);
-      for (int j0 = kWave; j0 < a.b.B; j0 += kWave) {
-        const Seq t = seq_of(a, j0 + lane);
-        n += t.tiles * ranges_of(t, chunk);
-      }
-      all = uni(wave_sum((float)n)) * groups;
+      all = sum([chunk](int t, int n) { return (float)(t * ranges_of(n, chunk)); }) * groups;
       if (all <= room) break;
       if (k < 2) chunk = ((int)min((float)chunk * all / room, 1e9f) + 128) & ~127;
     }
     const float c = ceilf(all / (float)a.own.target) * (float)(chunk + kRangeCost);
     if (c < cost) cost = c, best = chunk;
+    if (chunk <= (heads > 1 ? 128 : a.own.least)) break;
   }
   return Cut{best, heads};
+}
+// The cut and every sequence's first item, for the kernels that come after; by one wave
+__device__ __forceinline__ void write_plan(const AttnArgs& a, const Seq& s0, Cut cut, int lane) {
+  if (lane == 0) a.plan[0] = cut.chunk, a.plan[1] = cut.heads;
+  int run = 0;
+  for (int j0 = 0; j0 < a.b.B; j0 += kWave) {
+    const Seq t = j0 ? seq_of(a, j0 + lane) : s0;
+    const int mine = t.tiles * ranges_of(t.len, cut.chunk), upto = run + wave_scan(mine);
+    if (j0 + lane < a.b.B) a.plan[4 + j0 + lane] = upto - mine;
+    run = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+// At a kernel's start: the cut of the sequences' own tokens. Behind a prefix its kernel's last workgroup has made it; without one
+// every workgroup makes it and the first leaves it for k_combine.
+__device__ __forceinline__ bool begin_plan(const AttnArgs& a, int prefix, int lane, int wave, Seq& s0, Cut& cut) {
+  if (prefix) {
+    if (blockIdx.x != gridDim.x - 1) return true;
+    if (wave == 0) s0 = seq_of(a, lane), write_plan(a, s0, own_plan(a, s0, lane), lane);
+    return false;
+  }
+  s0 = seq_of(a, lane);
+  if (a.pre.splits) {
+    cut = Cut{uni(a.plan[0]), uni(a.plan[1])};
+  } else {
+    cut = own_plan(a, s0, lane);
+    if (blockIdx.x == 0 && wave == 0 && a.own.target) write_plan(a, s0, cut, lane);
+  }
+  return true;
 }
 // The sequence that `item` (of all sequences' ranges times tiles) falls to, and how many items precede the sequence's; false past the last
 __device__ __forceinline__ bool own_find(const AttnArgs& a, const Seq& s0, int chunk, int item, int lane, Seq& s, int& b, int& before) {
   int run = 0;
   for (int j0 = 0; j0 < a.b.B; j0 += kWave) {
     const Seq t = j0 ? seq_of(a, j0 + lane) : s0;
-    const int mine = t.tiles * ranges_of(t, chunk), upto = run + wave_scan(mine);
+    const int mine = t.tiles * ranges_of(t.len, chunk), upto = run + wave_scan(mine);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > item);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -166,7 +206,7 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, const Seq& s0, Cut c
   const int n = item / groups, i = n - before, split = i / s.tiles, head = item % groups * cut.heads;
   if ((int64_t)(n + 1) * a.c.Hkv > a.own.most) return false;
   t = Item{(table_t)(uintptr_t)(a.b.table + (size_t)b * a.b.table_ld), head, s.first, s.rows, s.len, split * chunk, (int)min((int64_t)s.len, (int64_t)(split + 1) * chunk), i % s.tiles,
-           own_places(a) + ((int64_t)n * a.c.Hkv + head) * a.own.cols, a.own.cols, true, a.pre.splits == 0 && ranges_of(s, chunk) == 1};
+           own_places(a) + ((int64_t)n * a.c.Hkv + head) * a.own.cols, a.own.cols, true, a.pre.splits == 0 && ranges_of(s.len, chunk) == 1};
   return true;
 }
 
@@ -413,7 +453,7 @@ __global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(
   float *red_m = lds + 4 * COLS * LD, *red_l = red_m + 4 * COLS;
   Seq s0{};
   Cut cut{0, a.pre.heads};
-  if (!prefix) s0 = seq_of(a, lane), cut = own_plan(a, s0, lane);
+  if (!begin_plan(a, prefix, lane, wave, s0, cut)) return;
   for (int item = blockIdx.x;; item += gridDim.x) {
     Item it;
     if (prefix) {
@@ -715,7 +755,7 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
   const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
   Seq s0{};
   Cut cut{0, a.pre.heads};
-  if (!prefix) s0 = seq_of(a, lane), cut = own_plan(a, s0, lane);
+  if (!begin_plan(a, prefix, lane, wave, s0, cut)) return;
   for (int item = blockIdx.x;; item += gridDim.x) {
     Item it;
     if (prefix) {
@@ -938,24 +978,22 @@ __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
   __shared__ v4f_t racc[4][LR];
   __shared__ float rl[4], rm[4];
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), part = wave % WPH, r = blockIdx.x, head = (int)blockIdx.y * (4 / WPH) + wave / WPH;
-  const Seq s0 = seq_of(a, lane);
-  const int chunk = own_plan(a, s0, lane).chunk;
+  const int chunk = uni(a.plan[0]);
   // the row's sequence
   Seq s{0, 0, 0, 0};
-  int before = 0, run = 0;
+  int before = 0;
   bool found = false;
   for (int j0 = 0; j0 < a.b.B && !found; j0 += kWave) {
-    const Seq t = j0 ? seq_of(a, j0 + lane) : s0;
-    const int mine = t.tiles * ranges_of(t, chunk), upto = run + wave_scan(mine);
+    const Seq t = seq_of(a, j0 + lane);
+    const int first = j0 + lane < a.b.B ? a.plan[4 + j0 + lane] : 0;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(t.rows > 0 && t.first <= r && r < t.first + t.rows);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      before = __builtin_amdgcn_readlane(upto - mine, l), found = true;
+      before = __builtin_amdgcn_readlane(first, l), found = true;
       s = Seq{__builtin_amdgcn_readlane(t.first, l), __builtin_amdgcn_readlane(t.rows, l), __builtin_amdgcn_readlane(t.len, l), __builtin_amdgcn_readlane(t.tiles, l)};
     }
-    run = __builtin_amdgcn_readlane(upto, 63);
   }
-  const int own = ranges_of(s, chunk);
+  const int own = ranges_of(s.len, chunk);
   if (!found || (a.pre.splits == 0 && own == 1)) return;  // (the same for the whole workgroup)
   const bool live = head < a.Hq;
   const int h = (live ? head : 0) / a.G, px = r * a.G + head % a.G, ox = (r - s.first) * a.G + head % a.G;
@@ -1036,7 +1074,7 @@ struct Layout {
   Part pre;
   Own own;
   int own_grid;
-  size_t ml, part;  // bytes
+  size_t ml, part, plan;  // bytes
 };
 Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
   const int G = Hq / c.Hkv, cus = num_cus_cached();
@@ -1062,7 +1100,7 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
   y.own.most = (int)std::min<int64_t>(most, 1 << 30);
   y.own_grid = (int)std::min<int64_t>(room, most);
   slots += (int64_t)y.own.most * y.own.cols;
-  y.ml = align256((size_t)slots * sizeof(float2)), y.part = align256((size_t)slots * c.D * 4);
+  y.ml = align256((size_t)slots * sizeof(float2)), y.part = align256((size_t)slots * c.D * 4), y.plan = align256((size_t)(b.B + 4) * 4);
   return y;
 }
 
@@ -1080,7 +1118,7 @@ template <int D, bool F8>
 int launch(const AttnArgs& a, const Layout& y, hipStream_t st) {
   if (a.pre.splits) {
     const int64_t pairs = (int64_t)a.pre.splits * (a.c.Hkv / a.pre.heads);
-    if (int rc = launch_part<D, F8>(a, y.kp, (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles), 1, st)) return rc;
+    if (int rc = launch_part<D, F8>(a, y.kp, (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles + 1), 1, st)) return rc;
   }
   if (int rc = launch_part<D, F8>(a, y.ko, (unsigned)y.own_grid, 0, st)) return rc;
   if (!a.pre.splits && !a.own.target) return DSGX_OK;
@@ -1107,7 +1145,7 @@ using namespace dsgx;
 extern "C" size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, int Hq) {
   if (check(cache, batch, Hq)) return 0;
   const Layout y = make_layout(*cache, *batch, Hq);
-  return y.ml + y.part;
+  return y.ml + y.part + y.plan;
 }
 
 extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale, uint16_t* out, int64_t ldo,
@@ -1126,6 +1164,7 @@ extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch,
   a.scale2 = scale == 0.f ? 1.f : std::fabs(scale) * kLog2e, a.q_flip = scale < 0.f ? 0x80008000u : 0u, a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu;
   a.ml = static_cast<float2*>(ws);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + y.ml);
+  a.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + y.ml + y.part);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f8 = cache->fmt == DSGX_KV_E4M3;
   switch (cache->D) {
