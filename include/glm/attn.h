@@ -1,6 +1,7 @@
 // glm:: - the dense GEMV operators with the reference engine's names and argument order
 // (altar1-4xgx10-switchless/engine/attn/attn.h:59-158), forwarding to the C ABI in dsgx.h. Only the weight-streaming
-// GEMV, its many-row form gemm() and dequant_int4 are on this build's path; the attention side of attn.h is not mirrored.
+// GEMV, its many-row form gemm() and dequant_int4 are on this build's path; the attention side of attn.h is not mirrored (whole heads over a
+// paged cache: dsgx_kv_append and dsgx_attn).
 #pragma once
 #include <cstddef>
 #include <cstdint>
