@@ -1,9 +1,11 @@
 """lib.spec_verify against the definition in f64 (tokens and counts equal), and the distribution that it draws from."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
-from dsgx10_amd import lib
+from dsgx10_amd import abi, lib
 from tests import kv
 
 pytestmark = pytest.mark.gpu
@@ -177,3 +179,52 @@ def test_captured_call_replays_on_new_numbers():
         want = _want(d)
         assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(accepted.cpu().numpy(), want[1])
         assert np.array_equal(_call(d, ws=ws)[0], want[0])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "prob"])
+@pytest.mark.parametrize("rows,V", [([3] * 40, 70001), ([4, 1, 7] * 100, 9000), ([2], 200003)])
+def test_pieces_of_several_chunks(rows, V, kind):
+    d = _inputs(rows, V, kind, 77, False, None if kind == "prob" else [0.0 if b % 5 == 1 else 0.9 for b in range(len(rows))])
+    if kind != "prob":
+        # a maximum that rises from chunk to chunk, and a first chunk that holds nothing
+        d["target"] += torch.arange(V) // 4096 * 0.125
+        d["target"][1::2, :4096] = -float("inf")
+    _check(d)
+
+
+@pytest.mark.parametrize("where", [5, 69000])
+def test_a_nan_or_infinity_in_any_chunk_refuses_the_row(where):
+    rows = [3] * 40
+    for value in (float("nan"), float("inf")):
+        d = _inputs(rows, 70001, "f32", 78, True, [0.7] * 40)
+        d["target"][0, where] = value
+        tokens, accepted = _call(d)
+        assert accepted[0] == 0 and tokens[0] == -1
+        want = _want({**d, "target": d["target"].nan_to_num(0.0, posinf=0.0)})
+        assert np.array_equal(tokens[3:], want[0][3:]) and np.array_equal(accepted[1:], want[1][1:])
+
+
+@pytest.mark.parametrize("T", [1e-3, 1e-6, 3e-9, 1e-10, 1e-30, 1e-44])
+def test_temperatures_near_zero(T):
+    """down to where 700 T is less than a step of the maximum; then only the largest logits' ids are left, evenly"""
+    d = _inputs([3, 2, 4], 6000, "f32", 79, False, [T] * 3)
+    d["target"][2, [7, 4500]] = 30.0
+    _check(d)
+
+
+@pytest.mark.parametrize("T", [1e6, 1e30, 3e38])
+def test_temperatures_that_flatten_everything(T):
+    d = _inputs([3, 2, 4], 6000, "f32", 80, False, [T] * 3)
+    d["target"][:, 100:4500] = -float("inf")
+    _check(d)
+
+
+def test_no_rows_at_all():
+    z = lambda n, t=torch.float32: torch.zeros(n, dtype=t, device="cuda")  # noqa: E731
+    ids, ws = z(4, torch.int32), z(lib.spec_verify_ws_bytes(3, 0, 500), torch.uint8)
+    for kind in (torch.float32, torch.bfloat16):
+        accepted = torch.full((3,), 9, dtype=torch.int32, device="cuda")
+        a = abi.VerifyIn(z(500, kind).data_ptr(), None, ids.data_ptr(), ids.data_ptr(), z(4).data_ptr(), z(3).data_ptr(), None, 500, 500, int(kind == torch.bfloat16), 500, 3, 0, 2)
+        assert lib.lib().dsgx_spec_verify(C.byref(a), ids.data_ptr(), accepted.data_ptr(), ws.data_ptr(), None) == abi.OK
+        torch.cuda.synchronize()
+        assert accepted.tolist() == [0, 0, 0] and ids.tolist() == [0] * 4
