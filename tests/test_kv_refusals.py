@@ -92,3 +92,10 @@ def test_python_handles_refuse_what_is_no_cache():
     for bad in (dict(lens=lens.long()), dict(table=table[:, ::2]), dict(cu_rows=lens.float())):
         with pytest.raises(lib.DsgxError):
             lib.kv_batch(2, 1, 10, bad.get("lens", lens), bad.get("table", table), cu_rows=bad.get("cu_rows"))
+
+
+def test_packed_arguments_are_the_structs():
+    a = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, -13, 14, 15, 1, 17, 0.5)
+    assert lib._APPEND(*a) == bytes(abi.KvAppendIn(*a))
+    a = (1, 2, 3, 4, 5, 6, 7, 8, 1 << 40, 2, -11, 12, 13, 14)
+    assert lib._VERIFY(*a) == bytes(abi.VerifyIn(*a))
