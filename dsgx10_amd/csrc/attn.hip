@@ -38,6 +38,7 @@ struct AttnArgs {
   uint16_t* out;
   float *lse, *part;  // part: [places][cols][D], the prefix's first
   float2* ml;         // [places][cols]
+  int pre_blocks;     // of a launch for both
   int32_t* plan;      // [4 + B]: tokens a range, heads a workgroup; from 4 on every sequence's first item
   int64_t ldq, ldo;
   int Hq, G, page_shift;
@@ -139,20 +140,31 @@ __device__ __forceinline__ void write_plan(const AttnArgs& a, const Seq& s0, Cut
     run = __builtin_amdgcn_readlane(upto, 63);
   }
 }
-// At a kernel's start: the cut of the sequences' own tokens. Behind a prefix its kernel's last workgroup has made it; without one
-// every workgroup makes it and the first leaves it for k_combine.
-__device__ __forceinline__ bool begin_plan(const AttnArgs& a, int prefix, int lane, int wave, Seq& s0, Cut& cut) {
-  if (prefix) {
-    if (blockIdx.x != gridDim.x - 1) return true;
+// What a workgroup of a launch is: `block` of `blocks` for the prefix or for the sequences' own tokens
+enum Mode { kOwnOnly, kPrefixOnly, kBoth };
+struct Role {
+  bool prefix;
+  int block, blocks;
+};
+// kBoth: the prefix's first, which are the longer ones (in turn with the others, 32768 tokens under 300 rows of 32 heads took 367 us instead of 250)
+__device__ __forceinline__ Role role_of(const AttnArgs& a, int mode) {
+  const int i = blockIdx.x, pre = mode == kBoth ? a.pre_blocks : mode == kPrefixOnly ? (int)gridDim.x : 0;
+  return i < pre ? Role{true, i, pre} : Role{false, i - pre, (int)gridDim.x - pre};
+}
+// At a kernel's start: the cut of the sequences' own tokens. Where the prefix has a launch of its own before theirs, its last workgroup has made
+// it; else every workgroup makes it and the first leaves it for k_combine.
+__device__ __forceinline__ bool begin_plan(const AttnArgs& a, int mode, const Role& role, int lane, int wave, Seq& s0, Cut& cut) {
+  if (role.prefix) {
+    if (mode == kBoth || role.block != role.blocks - 1) return true;
     if (wave == 0) s0 = seq_of(a, lane), write_plan(a, s0, own_plan(a, s0, lane), lane);
     return false;
   }
   s0 = seq_of(a, lane);
-  if (a.pre.splits) {
+  if (a.pre.splits && mode != kBoth) {
     cut = Cut{uni(a.plan[0]), uni(a.plan[1])};
   } else {
     cut = own_plan(a, s0, lane);
-    if (blockIdx.x == 0 && wave == 0 && a.own.target) write_plan(a, s0, cut, lane);
+    if (role.block == 0 && wave == 0 && a.own.target) write_plan(a, s0, cut, lane);
   }
   return true;
 }
@@ -188,9 +200,9 @@ __device__ __forceinline__ Item uniform(const Item& t) {
   return Item{(table_t)uni64((int64_t)t.tab), uni(t.head), uni(t.first), uni(t.rows), uni(t.len), uni(t.lo), uni(t.hi), uni(t.tile), uni64(t.place), uni64(t.next), uni((int)t.causal) != 0,
               uni((int)t.alone) != 0};
 }
-__device__ __forceinline__ Item prefix_item(const AttnArgs& a, bool& any) {
+__device__ __forceinline__ Item prefix_item(const AttnArgs& a, int i, bool& any) {
   // The tiles that read the same tokens run on the same XCD (workgroup i runs on XCD i % 8) next to each other, out of its L2
-  const int i = blockIdx.x, pair = i / 8 / a.pre.tiles * 8 + i % 8, groups = a.c.Hkv / a.pre.heads, split = pair / groups;
+  const int pair = i / 8 / a.pre.tiles * 8 + i % 8, groups = a.c.Hkv / a.pre.heads, split = pair / groups;
   Item t{(table_t)(uintptr_t)a.b.prefix, pair % groups * a.pre.heads, 0, a.b.rows, a.b.prefix_len, split * a.pre.chunk, 0, i / 8 % a.pre.tiles, 0, 0, false, false};
   t.hi = min(t.len, t.lo + a.pre.chunk), t.next = (int64_t)a.pre.tiles * a.pre.cols;
   t.place = (int64_t)(split * a.c.Hkv + t.head) * t.next + (int64_t)t.tile * a.pre.cols;
@@ -443,22 +455,24 @@ template <int D, bool F8, int NQ>
 constexpr int kNarrowDepth = D == 64 ? (NQ == 2 ? 1 : F8 ? 3 : 2) : D == 128 ? (F8 ? (NQ == 1 ? 3 : 2) : NQ == 1 ? 2 : 1) : 1;
 
 template <int D, bool F8, int NQ>
-__global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(AttnArgs a, int prefix) {
+__device__ __forceinline__ void narrow(const AttnArgs& a, int mode, const Role& role) {
+  const bool prefix = role.prefix;
   using N = Narrow<D, F8, NQ>;
   constexpr int VL = N::VL, LD = D + 4, COLS = 16 * NQ;
-  extern __shared__ float lds[];  // [4][COLS][LD] outputs, then [4][COLS] maxima and sums
+  extern __shared__ __align__(16) uint8_t tiles[];
+  float* lds = reinterpret_cast<float*>(tiles);  // [4][COLS][LD] outputs, then [4][COLS] maxima and sums
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), g = lane >> 4, col = lane & 15, G = a.G;
   constexpr int esz = F8 ? 1 : 2;
   const uint32_t ts = (uint32_t)(a.c.tok_stride * esz), ko = col * ts + 16 * g, vo = 4 * g * ts + col * N::VW * 4;
   float *red_m = lds + 4 * COLS * LD, *red_l = red_m + 4 * COLS;
   Seq s0{};
   Cut cut{0, a.pre.heads};
-  if (!begin_plan(a, prefix, lane, wave, s0, cut)) return;
-  for (int item = blockIdx.x;; item += gridDim.x) {
+  if (!begin_plan(a, mode, role, lane, wave, s0, cut)) return;
+  for (int item = role.block;; item += role.blocks) {
     Item it;
     if (prefix) {
       bool any;
-      it = prefix_item(a, any);
+      it = prefix_item(a, role.block, any);
       if (!any) return;
     } else if (!own_item(a, s0, cut, item, lane, it)) {
       return;
@@ -743,7 +757,8 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 template <int D, bool F8, int QW>
-__global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide(AttnArgs a, int prefix) {
+__device__ __forceinline__ void wide(const AttnArgs& a, int mode, const Role& role) {
+  const bool prefix = role.prefix;
   using W = Wide<D, F8, QW>;
   using acc_t = typename W::acc_t;
   constexpr int KV = W::KV, COLS = 4 * QW;
@@ -755,12 +770,12 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
   const uint32_t ts = (uint32_t)(a.c.tok_stride * esz);
   Seq s0{};
   Cut cut{0, a.pre.heads};
-  if (!begin_plan(a, prefix, lane, wave, s0, cut)) return;
-  for (int item = blockIdx.x;; item += gridDim.x) {
+  if (!begin_plan(a, mode, role, lane, wave, s0, cut)) return;
+  for (int item = role.block;; item += role.blocks) {
     Item it;
     if (prefix) {
       bool any;
-      it = prefix_item(a, any);
+      it = prefix_item(a, role.block, any);
       if (!any) return;
     } else if (!own_item(a, s0, cut, item, lane, it)) {
       return;
@@ -971,6 +986,22 @@ __global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide
   }
 }
 
+template <int D, bool F8, int NQ>
+__global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(AttnArgs a, int mode) {
+  narrow<D, F8, NQ>(a, mode, role_of(a, mode));
+}
+template <int D, bool F8, int QW>
+__global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide(AttnArgs a, int mode) {
+  wide<D, F8, QW>(a, mode, role_of(a, mode));
+}
+// The prefix with 128 columns a workgroup and the sequences' own tokens with 16 NQ, in one launch
+template <int D, bool F8, int NQ>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_attn_both(AttnArgs a) {
+  const Role role = role_of(a, kBoth);
+  if (role.prefix) wide<D, F8, 32>(a, kBoth, role);
+  else narrow<D, F8, NQ>(a, kBoth, role);
+}
+
 // The ranges' outputs of a row's head joined by their maxima: WPH waves a head, D / 4 lanes a range
 template <int D, int WPH>
 __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
@@ -1074,6 +1105,7 @@ struct Layout {
   Part pre;
   Own own;
   int own_grid;
+  bool both;  // prefix and own tokens in one launch
   size_t ml, part, plan;  // bytes
 };
 Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
@@ -1081,19 +1113,34 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
   const bool f8 = c.fmt == DSGX_KV_E4M3;
   Layout y{};
   int64_t slots = 0;
+  y.ko = kind_of((int64_t)b.max_rows * G, c.D);
+  if (b.prefix_len) {
+    y.kp = kind_of((int64_t)b.rows * G, c.D);
+    // A wider form than the columns ask for, so that one launch can have both. Own tokens of 12 x 2 rows by 32 columns behind 3000 tokens: 40.4 us in
+    // two launches, 27.2 in one. The prefix by 128 columns for 56: 3000 tokens 25.0 us, 14.3; 25000 41.4, 33.0 (e4m3 34.6, 27.4); 60000 70.0, 68.9
+    // (e4m3 52.2, 61.8).
+    if (y.kp == kNarrow32 && b.max_len <= 32768) y.ko = kNarrow32;
+    if (y.kp == kWide64 && y.ko <= kNarrow32 && b.prefix_len <= 32768) y.kp = kWide128;
+  }
+  y.own.cols = cols_of(y.ko), y.own.heads = heads_of(y.ko, c);
+  int room = cus * resident(y.ko, c.D, f8);
   if (b.prefix_len) {
     const int64_t cols = (int64_t)b.rows * G;
-    y.kp = kind_of(cols, c.D);
     y.pre.cols = cols_of(y.kp), y.pre.tiles = (int)((cols + y.pre.cols - 1) / y.pre.cols);
     y.pre.heads = heads_of(y.kp, c);
-    const int64_t each = (int64_t)(c.Hkv / y.pre.heads) * y.pre.tiles, room = (int64_t)cus * resident(y.kp, c.D, f8);
-    y.pre.chunk = std::max(256, round_up((b.prefix_len + room / each) / std::max<int64_t>(1, room / each), 128));
+    const int64_t each = (int64_t)(c.Hkv / y.pre.heads) * y.pre.tiles;
+    y.both = y.kp == y.ko || (y.kp == kWide128 && y.ko <= kNarrow32);
+    double pre_room = cus * resident(y.kp, c.D, f8);
+    // In one launch the room is shared by the work (tokens times tiles; of max_len half, on average), two thirds at least for the prefix, whose
+    // ranges are cut here; what is left of it is the own tokens', or all of it where they are most of the work and come second.
+    const double mine = 0.5 * b.B * b.max_len * (((int64_t)b.max_rows * G + y.own.cols - 1) / y.own.cols), theirs = (double)b.prefix_len * y.pre.tiles;
+    if (y.both) room = std::min(room, (int)pre_room), pre_room = room * std::max(2. / 3, theirs / (theirs + mine));
+    const int64_t splits = std::max<int64_t>(1, (int64_t)(pre_room / each + (y.both ? 0.5 : 0)));
+    y.pre.chunk = std::max(256, round_up((b.prefix_len + splits) / splits, 128));
     y.pre.splits = (b.prefix_len + y.pre.chunk - 1) / y.pre.chunk;
     slots = each * y.pre.heads * y.pre.splits * y.pre.cols;
+    if (y.both && mine < 2 * theirs) room = (int)std::max((int64_t)room / 3, room - each * y.pre.splits);
   }
-  y.ko = kind_of((int64_t)b.max_rows * G, c.D);
-  y.own.cols = cols_of(y.ko), y.own.heads = heads_of(y.ko, c);
-  const int room = cus * resident(y.ko, c.D, f8);
   // short contexts without a prefix: a range a sequence, which leaves nothing to join
   y.own.target = !b.prefix_len && b.max_len <= 512 ? 0 : room, y.own.least = 256;
   const int64_t most = 4 * (int64_t)y.own.target * y.own.heads + (int64_t)c.Hkv * (((int64_t)b.rows * G) / y.own.cols + b.B + 1);
@@ -1105,22 +1152,43 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
 }
 
 template <int D, bool F8>
-int launch_part(const AttnArgs& a, Kind k, unsigned grid, int prefix, hipStream_t st) {
-  const int cols = cols_of(k);
-  const size_t lds = k <= kNarrow32 ? (size_t)(4 * cols * (D + 4) + 8 * cols) * 4 : 4 * Wide<D, F8, 32>::kTile;
+size_t lds_of(Kind k) {
+  return k <= kNarrow32 ? (size_t)(4 * cols_of(k) * (D + 4) + 8 * cols_of(k)) * 4 : 4 * Wide<D, F8, 32>::kTile;
+}
+template <int D, bool F8>
+int launch_part(const AttnArgs& a, Kind k, unsigned grid, Mode mode, hipStream_t st) {
+  const size_t lds = lds_of<D, F8>(k);
   auto kern = k == kNarrow16 ? k_attn_narrow<D, F8, 1> : k == kNarrow32 && D < 256 ? k_attn_narrow<(D < 256 ? D : 64), F8, 2> : k == kWide64 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
   if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, st, a, prefix);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, st, a, (int)mode);
   DSGX_HIP(hipGetLastError());
   return DSGX_OK;
 }
+// One launch for prefix and own tokens where one kernel has both their forms: a launch's ramp and its first chain of loads take about 10 us.
+// 8011 tokens before 48 rows of 64 heads: 49.9 us in two launches, 35.7 in one; 32768 before 300 of 32 (e4m3): 262, 240; 5000 before 2 of 32: 31.4, 20.0;
+// 9000 before 20 of 16 heads of 256 over one: 45.9, 26.0.
 template <int D, bool F8>
-int launch(const AttnArgs& a, const Layout& y, hipStream_t st) {
+int launch(AttnArgs& a, const Layout& y, hipStream_t st) {
+  const unsigned own = ((unsigned)y.own_grid + 7) / 8 * 8;  // (more than there are items do nothing)
   if (a.pre.splits) {
     const int64_t pairs = (int64_t)a.pre.splits * (a.c.Hkv / a.pre.heads);
-    if (int rc = launch_part<D, F8>(a, y.kp, (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles + 1), 1, st)) return rc;
+    const unsigned pre = (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles);
+    a.pre_blocks = (int)pre;
+    if (y.kp == y.ko) {
+      if (int rc = launch_part<D, F8>(a, y.kp, pre + own, kBoth, st)) return rc;
+    } else if (y.kp == kWide128 && y.ko <= kNarrow32) {
+      const size_t lds = std::max(lds_of<D, F8>(y.kp), lds_of<D, F8>(y.ko));
+      auto kern = y.ko == kNarrow16 ? k_attn_both<D, F8, 1> : k_attn_both<(D < 256 ? D : 64), F8, 2>;
+      if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
+      hipLaunchKernelGGL(kern, dim3(pre + own), dim3(256), lds, st, a);
+      DSGX_HIP(hipGetLastError());
+    } else {
+      if (int rc = launch_part<D, F8>(a, y.kp, pre + 1, kPrefixOnly, st)) return rc;
+      if (int rc = launch_part<D, F8>(a, y.ko, own, kOwnOnly, st)) return rc;
+    }
+  } else {
+    if (int rc = launch_part<D, F8>(a, y.ko, own, kOwnOnly, st)) return rc;
   }
-  if (int rc = launch_part<D, F8>(a, y.ko, (unsigned)y.own_grid, 0, st)) return rc;
   if (!a.pre.splits && !a.own.target) return DSGX_OK;
   if ((int64_t)a.b.rows * a.Hq <= 1024) hipLaunchKernelGGL((k_combine<D, 4>), dim3(a.b.rows, a.Hq), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_combine<D, 1>), dim3(a.b.rows, (a.Hq + 3) / 4), dim3(256), 0, st, a);

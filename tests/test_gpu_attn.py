@@ -32,6 +32,14 @@ def test_prefix(prefix, Hq, Hkv, D, fmt):
     kv.check_attn(s, *s.run())
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("B,n,G,max_len", [(9, 1, 8, None), (5, 3, 8, None), (4, 1, 16, 40000), (3, 1, 8, 1), (1, 2, 4, None), (2, 8, 8, None), (1, 12, 8, 9000), (1, 6, 8, None)])
+def test_prefix_and_own_tokens_by_every_pair_of_kernels(B, n, G, max_len, D, fmt):
+    s = kv.Step([n] * B, [n + (37 * b) % 290 for b in range(B)], prefix=700, Hq=2 * G, Hkv=2, D=D, fmt=fmt, page=16, seed=B + n, max_len=max_len)
+    kv.check_attn(s, *s.run())
+
+
 @pytest.mark.parametrize("B,n", [(1, 1), (3, 7), (40, 1), (70, 2), (130, 4)])
 def test_many_rows_behind_a_prefix(B, n):
     s = kv.Step([n] * B, [n + (7 * b) % 50 for b in range(B)], prefix=333, Hq=16, Hkv=2, D=128, page=16, seed=B)
