@@ -450,7 +450,7 @@ struct Narrow {
 
 // Waves a SIMD that the registers leave room for, and blocks on their way a wave
 template <int D, bool F8, int NQ>
-constexpr int kNarrowWaves = D == 64 ? 3 : D == 128 ? 2 : F8 ? 2 : 1;
+constexpr int kNarrowWaves = D == 64 ? 3 : 2;
 template <int D, bool F8, int NQ>
 constexpr int kNarrowDepth = D == 64 ? (NQ == 2 ? 1 : F8 ? 3 : 2) : D == 128 ? (F8 ? (NQ == 1 ? 3 : 2) : NQ == 1 ? 2 : 1) : 1;
 
@@ -618,7 +618,7 @@ __device__ __forceinline__ void narrow(const AttnArgs& a, int mode, const Role& 
 // values a thread, a byte permutation a pair), so that both operands are 16-byte reads from LDS. Layouts (chunks of 16 bytes): K as rows of
 // a token, V as rows of a d whose chunks hold the eight tokens that one lane's scores belong to, so that the scores are the second
 // product's operand as they stand; the chunks of a row are XORed with its number, which spreads sixteen lanes' rows over all banks.
-// QW 32: v_mfma_f32_32x32x16_bf16, 128 columns a workgroup; QW 16: v_mfma_f32_16x16x32_bf16, 64 columns.
+// QW 32 (D 64, 128): v_mfma_f32_32x32x16_bf16, 128 columns a workgroup; QW 16: v_mfma_f32_16x16x32_bf16, 64 columns.
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 
 // a barrier for what passes through LDS alone: loads from memory stay on their way
@@ -991,12 +991,12 @@ __global__ void __launch_bounds__(256, (kNarrowWaves<D, F8, NQ>)) k_attn_narrow(
   narrow<D, F8, NQ>(a, mode, role_of(a, mode));
 }
 template <int D, bool F8, int QW>
-__global__ void __launch_bounds__(256, D == 256 && QW == 32 ? 1 : 2) k_attn_wide(AttnArgs a, int mode) {
+__global__ void __launch_bounds__(256, 2) k_attn_wide(AttnArgs a, int mode) {
   wide<D, F8, QW>(a, mode, role_of(a, mode));
 }
 // The prefix with 128 columns a workgroup and the sequences' own tokens with 16 NQ, in one launch
 template <int D, bool F8, int NQ>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_attn_both(AttnArgs a) {
+__global__ void __launch_bounds__(256, 2) k_attn_both(AttnArgs a) {
   const Role role = role_of(a, kBoth);
   if (role.prefix) wide<D, F8, 32>(a, kBoth, role);
   else narrow<D, F8, NQ>(a, kBoth, role);
@@ -1085,14 +1085,21 @@ __global__ void __launch_bounds__(256) k_combine(AttnArgs a) {
 
 int round_up(int64_t v, int m) { return (int)((v + m - 1) / m * m); }
 
-// How `cols` query columns over the same tokens are worked on: 16 or 32 a workgroup from registers, 64 or 128 over tiles in LDS
+// How `cols` query columns over the same tokens are worked on: 16 or 32 a workgroup from registers, 64 or 128 over tiles in LDS.
+// 128 against 64, D 128: 6 x 8 rows of 16 heads over each of 4, 5000 to 8000 tokens 33.5 us, 37.2; 8011 tokens before 48 rows of 64 heads over 8 28.8, 36.2.
+// D 256 by 128 columns takes over half a SIMD's registers, and its one wave a SIMD waits for whatever it waits for: 5 rows of 64 heads over one, 50001
+// tokens 53.2 us (e4m3 51.9), by 64 columns 50.1 (43.0); 20000 before 300 rows of 32 heads 688 (680), 566 (539). By 16 from registers it is so
+// too for BF16: 16 rows of 8 heads over each of 2, 300 to 8000 tokens 28.7 us, by 64 columns 23.5 (e4m3 18.0, 22.8); and behind a prefix one launch
+// has both.
 enum Kind { kNarrow16, kNarrow32, kWide64, kWide128 };
-Kind kind_of(int64_t cols, int D) { return cols <= 16 ? kNarrow16 : cols <= 32 && D < 256 ? kNarrow32 : cols <= 64 ? kWide64 : kWide128; }
+Kind kind_of(int64_t cols, int D, bool f8, bool prefix) {
+  if (D == 256) return cols <= 16 && f8 && !prefix ? kNarrow16 : kWide64;
+  return cols <= 16 ? kNarrow16 : cols <= 32 ? kNarrow32 : cols <= 64 ? kWide64 : kWide128;
+}
 int cols_of(Kind k) { return 16 << k; }
 // workgroups a CU holds
-int resident(Kind k, int D, bool f8) {
-  if (k <= kNarrow32) return D == 64 ? 3 : D == 128 || f8 ? 2 : 1;
-  return D == 256 && k == kWide128 ? 1 : 2;
+int resident(Kind k, int D) {
+  return k <= kNarrow32 && D == 64 ? 3 : 2;
 }
 
 // Heads side by side a workgroup of the register kernels: their tokens' rows are neighbours in the usual layout of a page
@@ -1113,9 +1120,9 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
   const bool f8 = c.fmt == DSGX_KV_E4M3;
   Layout y{};
   int64_t slots = 0;
-  y.ko = kind_of((int64_t)b.max_rows * G, c.D);
+  y.ko = kind_of((int64_t)b.max_rows * G, c.D, f8, b.prefix_len > 0);
   if (b.prefix_len) {
-    y.kp = kind_of((int64_t)b.rows * G, c.D);
+    y.kp = kind_of((int64_t)b.rows * G, c.D, f8, true);
     // A wider form than the columns ask for, so that one launch can have both. Own tokens of 12 x 2 rows by 32 columns behind 3000 tokens: 40.4 us in
     // two launches, 27.2 in one. The prefix by 128 columns for 56: 3000 tokens 25.0 us, 14.3; 25000 41.4, 33.0 (e4m3 34.6, 27.4); 60000 70.0, 68.9
     // (e4m3 52.2, 61.8).
@@ -1123,14 +1130,14 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
     if (y.kp == kWide64 && y.ko <= kNarrow32 && b.prefix_len <= 32768) y.kp = kWide128;
   }
   y.own.cols = cols_of(y.ko), y.own.heads = heads_of(y.ko, c);
-  int room = cus * resident(y.ko, c.D, f8);
+  int room = cus * resident(y.ko, c.D);
   if (b.prefix_len) {
     const int64_t cols = (int64_t)b.rows * G;
     y.pre.cols = cols_of(y.kp), y.pre.tiles = (int)((cols + y.pre.cols - 1) / y.pre.cols);
     y.pre.heads = heads_of(y.kp, c);
     const int64_t each = (int64_t)(c.Hkv / y.pre.heads) * y.pre.tiles;
     y.both = y.kp == y.ko || (y.kp == kWide128 && y.ko <= kNarrow32);
-    double pre_room = cus * resident(y.kp, c.D, f8);
+    double pre_room = cus * resident(y.kp, c.D);
     // In one launch the room is shared by the work (tokens times tiles; of max_len half, on average), two thirds at least for the prefix, whose
     // ranges are cut here; what is left of it is the own tokens', or all of it where they are most of the work and come second.
     const double mine = 0.5 * b.B * b.max_len * (((int64_t)b.max_rows * G + y.own.cols - 1) / y.own.cols), theirs = (double)b.prefix_len * y.pre.tiles;
@@ -1153,20 +1160,34 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
 
 template <int D, bool F8>
 size_t lds_of(Kind k) {
-  return k <= kNarrow32 ? (size_t)(4 * cols_of(k) * (D + 4) + 8 * cols_of(k)) * 4 : 4 * Wide<D, F8, 32>::kTile;
+  return k <= kNarrow32 ? (size_t)(4 * cols_of(k) * (D + 4) + 8 * cols_of(k)) * 4 : 4 * Wide<D, F8, 16>::kTile;
 }
 template <int D, bool F8>
 int launch_part(const AttnArgs& a, Kind k, unsigned grid, Mode mode, hipStream_t st) {
   const size_t lds = lds_of<D, F8>(k);
-  auto kern = k == kNarrow16 ? k_attn_narrow<D, F8, 1> : k == kNarrow32 && D < 256 ? k_attn_narrow<(D < 256 ? D : 64), F8, 2> : k == kWide64 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
+  void (*kern)(AttnArgs, int);
+  if constexpr (D == 256 && F8) kern = k == kNarrow16 ? k_attn_narrow<D, F8, 1> : k_attn_wide<D, F8, 16>;
+  else if constexpr (D == 256) kern = k_attn_wide<D, F8, 16>;
+  else kern = k == kNarrow16 ? k_attn_narrow<D, F8, 1> : k == kNarrow32 ? k_attn_narrow<D, F8, 2> : k == kWide64 ? k_attn_wide<D, F8, 16> : k_attn_wide<D, F8, 32>;
   if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
   hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, st, a, (int)mode);
   DSGX_HIP(hipGetLastError());
   return DSGX_OK;
 }
+template <int D, bool F8>
+int launch_both(const AttnArgs& a, Kind ko, unsigned grid, hipStream_t st) {
+  if constexpr (D < 256) {
+    const size_t lds = std::max(lds_of<D, F8>(kWide128), lds_of<D, F8>(ko));
+    auto kern = ko == kNarrow16 ? k_attn_both<D, F8, 1> : k_attn_both<D, F8, 2>;
+    if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, st, a);
+    DSGX_HIP(hipGetLastError());
+  }
+  return DSGX_OK;
+}
 // One launch for prefix and own tokens where one kernel has both their forms: a launch's ramp and its first chain of loads take about 10 us.
 // 8011 tokens before 48 rows of 64 heads: 49.9 us in two launches, 35.7 in one; 32768 before 300 of 32 (e4m3): 262, 240; 5000 before 2 of 32: 31.4, 20.0;
-// 9000 before 20 of 16 heads of 256 over one: 45.9, 26.0.
+// 9000 before 20 of 16 heads of 256 over one: 45.9, 19.3.
 template <int D, bool F8>
 int launch(AttnArgs& a, const Layout& y, hipStream_t st) {
   const unsigned own = ((unsigned)y.own_grid + 7) / 8 * 8;  // (more than there are items do nothing)
@@ -1176,12 +1197,8 @@ int launch(AttnArgs& a, const Layout& y, hipStream_t st) {
     a.pre_blocks = (int)pre;
     if (y.kp == y.ko) {
       if (int rc = launch_part<D, F8>(a, y.kp, pre + own, kBoth, st)) return rc;
-    } else if (y.kp == kWide128 && y.ko <= kNarrow32) {
-      const size_t lds = std::max(lds_of<D, F8>(y.kp), lds_of<D, F8>(y.ko));
-      auto kern = y.ko == kNarrow16 ? k_attn_both<D, F8, 1> : k_attn_both<(D < 256 ? D : 64), F8, 2>;
-      if (int rc = allow_dynamic_lds((const void*)kern, lds)) return rc;
-      hipLaunchKernelGGL(kern, dim3(pre + own), dim3(256), lds, st, a);
-      DSGX_HIP(hipGetLastError());
+    } else if (y.both) {
+      if (int rc = launch_both<D, F8>(a, y.ko, pre + own, st)) return rc;
     } else {
       if (int rc = launch_part<D, F8>(a, y.kp, pre + 1, kPrefixOnly, st)) return rc;
       if (int rc = launch_part<D, F8>(a, y.ko, own, kOwnOnly, st)) return rc;
