@@ -214,3 +214,9 @@ def test_captured_step_replays_with_other_lengths():
         torch.cuda.synchronize()
         assert torch.equal(got, out.cpu()) and torch.equal(z, lse.cpu())
         s.lens, s.own_kv = full
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,L", [(64, 8, 8, 20011), (128, 8, 2, 12000), (256, 4, 1, 9000)])
+def test_one_row_over_many_ranges(D, Hq, Hkv, L):
+    s = kv.Step([1], [L], Hq=Hq, Hkv=Hkv, D=D, page=64, seed=D)
+    kv.check_attn(s, *s.run())
