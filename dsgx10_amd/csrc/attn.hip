@@ -1234,8 +1234,14 @@ using namespace dsgx;
 
 extern "C" size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, int Hq) {
   if (check(cache, batch, Hq)) return 0;
-  const Layout y = make_layout(*cache, *batch, Hq);
-  return y.ml + y.part + y.plan;
+  // At least every layout's, whatever lengths and prefix, and growing with sequences and rows: a program's largest batch sizes it. Columns of
+  // places: own items are 4 target + one a tile and sequence (own_plan's chunk is the work's share of the room at least), the prefix's
+  // workgroups the room + one a tile and head.
+  const int64_t cols = (int64_t)batch->rows * (Hq / cache->Hkv);
+  int64_t room = 0;
+  for (int k = kNarrow16; k <= kWide128; ++k) room = std::max(room, (int64_t)num_cus_cached() * resident((Kind)k, cache->D) * heads_of((Kind)k, *cache) * cols_of((Kind)k));
+  const size_t slots = (size_t)(5 * room + cache->Hkv * (2 * cols + ((int64_t)batch->B + 2) * cols_of(kWide128)));
+  return align256(slots * sizeof(float2)) + align256(slots * cache->D * 4) + align256((size_t)(batch->B + 4) * 4);
 }
 
 extern "C" int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale, uint16_t* out, int64_t ldo,

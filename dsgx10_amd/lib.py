@@ -10,7 +10,7 @@ from . import abi
 
 _SO = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", os.environ.get("DSGX_LIB", "libdsgx.so"))
 _lib = None
-_F32 = _TARGETS = None  # torch's f32; the kinds of spec_verify's logits by their dtype (set when the library is loaded)
+_F32 = _I32 = _TARGETS = None  # torch's types; the kinds of spec_verify's logits by their dtype (set when the library is loaded)
 _current = None  # () -> the current device's current stream, as the C ABI takes it (set when the library is loaded)
 
 
@@ -26,7 +26,7 @@ def so_path():
 
 def lib():
     """The loaded C ABI. Raises if the HIP extension has not been built (python -m dsgx10_amd.build)."""
-    global _lib, _current, _F32, _TARGETS
+    global _lib, _current, _F32, _I32, _TARGETS
     if _lib is None:
         import torch  # first: the library must bind to the HIP runtime torch's streams and buffers belong to
         if not os.path.exists(_SO):
@@ -93,7 +93,7 @@ def lib():
         # 2048 x 4096 takes the GPU 5.3 us, the call as a whole took 8.3)
         raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.cuda.current_device
         _current = (lambda: raw(device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
-        _F32, _TARGETS = torch.float32, {torch.float32: 0, torch.bfloat16: 1}
+        _F32, _I32, _TARGETS = torch.float32, torch.int32, {torch.float32: 0, torch.bfloat16: 1}
         _lib = L
     return _lib
 
@@ -318,21 +318,25 @@ _APPEND, _VERIFY = struct.Struct("8P4q5if").pack, struct.Struct("7P2q5i4x").pack
 def kv_append(cache, batch, k, ldk, v, ldv, q=None, ldq=0, Hq=0, q_out=None, ldqo=0, q_norm=None, k_norm=None, eps=1e-5, rope=None, rot=0, rot_off=0, pairs=False,
               pos=None, stream=None):
     """The step's rows on their way to attention: q and k normed per head and rotated, q to q_out, k and v into the cache"""
+    L = lib()
+    if (rope is not None and rope.dtype is not _F32) or (pos is not None and pos.dtype is not _I32):
+        raise DsgxError(abi.EINVAL, "kv_append: the table is f32, positions are i32")
     a = _APPEND(0 if q is None else q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), 0 if q_out is None else q_out.data_ptr(),
                 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), 0 if rope is None else rope.data_ptr(),
                 0 if pos is None else pos.data_ptr(), ldq, ldk, ldv, ldqo, Hq, rot, rot_off, int(pairs), 0 if rope is None else rope.numel() // max(rot, 1), eps)
-    rc = (_lib or lib()).dsgx_kv_append(C.byref(cache), C.byref(batch), a, _stream(stream))
+    rc = L.dsgx_kv_append(C.byref(cache), C.byref(batch), a, _stream(stream))
     if rc:
         _check(rc)
 
 
 def attn_ws_bytes(cache, batch, Hq):
+    """by the cache's shape, Hq, sequences and rows alone: that of the largest batch is enough for every one"""
     return lib().dsgx_attn_ws_bytes(C.byref(cache), C.byref(batch), Hq)
 
 
 def attn(cache, batch, q, ldq, Hq, scale, out, ldo, ws, lse=None, stream=None):
     """out = softmax(scale q K^T) V of the step's rows over the shared prefix and their sequences' own tokens; lse f32 [rows][Hq] optional"""
-    rc = (_lib or lib()).dsgx_attn(C.byref(cache), C.byref(batch), q.data_ptr(), ldq, Hq, scale, out.data_ptr(), ldo, 0 if lse is None else lse.data_ptr(), ws.data_ptr(),
+    rc = lib().dsgx_attn(C.byref(cache), C.byref(batch), q.data_ptr(), ldq, Hq, scale, out.data_ptr(), ldo, 0 if lse is None else lse.data_ptr(), ws.data_ptr(),
                                    _stream(stream))
     if rc:
         _check(rc)
@@ -348,6 +352,9 @@ def spec_verify(target, V, draft, u, us, tokens, accepted, ws, max_rows, cu_rows
     kind = 2 if probs and target.dtype is _F32 else _TARGETS.get(target.dtype) if not probs else None
     if kind is None or (q is not None and q.dtype is not _F32):
         raise DsgxError(abi.EINVAL, "spec_verify: a target of %s, a drafter's probabilities of %s" % (target.dtype, None if q is None else q.dtype))
+    if tokens.dtype is not _I32 or accepted.dtype is not _I32 or us.dtype is not _F32 or any(t is not None and t.dtype is not _I32 for t in (draft, cu_rows)) or \
+            any(t is not None and t.dtype is not _F32 for t in (u, temp)):
+        raise DsgxError(abi.EINVAL, "spec_verify: ids and bounds are i32, random numbers and temperatures f32")
     a = _VERIFY(target.data_ptr(), 0 if q is None else q.data_ptr(), 0 if draft is None else draft.data_ptr(), 0 if cu_rows is None else cu_rows.data_ptr(),
                 0 if u is None else u.data_ptr(), us.data_ptr(), 0 if temp is None else temp.data_ptr(), ldt or V, ldq or V, kind, V, accepted.numel(), tokens.numel(), max_rows)
     rc = L.dsgx_spec_verify(a, tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), _stream(stream))

@@ -381,7 +381,9 @@ DSGX_API int dsgx_kv_append(const dsgx_kv_cache* cache, const dsgx_kv_batch* bat
    A row that sees nothing has out 0 and lse -inf. What a masked or unwritten place holds (NaN, infinities) does not reach a result.
    Scores, softmax statistics and sums are f32; the softmax's numerators are rounded to bf16 for the matrix unit. q, out bf16
    [rows][ld*], a row's Hq heads of D side by side, 16-byte aligned. The prefix is read once for all rows. ws:
-   dsgx_attn_ws_bytes(...) bytes of device memory, zeroed once; it belongs to one call at a time (calls in stream order share it). */
+   dsgx_attn_ws_bytes(...) bytes of device memory; it belongs to one call at a time (calls in stream order share it). The size goes
+   by the cache's shape, Hq, B and rows alone and grows with the last two: that of the largest batch is enough for every one. scale is
+   finite (0: every token counts the same; negative: turned round). */
 DSGX_API size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, int Hq);
 DSGX_API int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale,
                        uint16_t* out, int64_t ldo, float* lse, void* ws, void* stream);
@@ -394,7 +396,8 @@ DSGX_API int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, c
    first that is not, the next token is drawn from max(p - q, 0) (all zero: from p), after the last from p: the lowest id v with
    sum(w[0 .. v]) > us[b] * sum(w). tokens [rows]: the accepted drafts, the drawn token, then -1; accepted [B].
    A draft outside 0 .. V - 1 is refused; a row whose weights have no finite positive sum draws -1 (its draft is refused).
-   kind 0: f32 logits, 1: bf16 logits, 2: f32 probabilities. temp null: 1. ws: dsgx_spec_verify_ws_bytes(...) bytes, zeroed once. */
+   kind 0: f32 logits, 1: bf16 logits, 2: f32 probabilities. temp null: 1. ws: dsgx_spec_verify_ws_bytes(...) bytes, zeroed
+   once; it belongs to one call at a time, and the largest call's is enough for every one. */
 typedef struct dsgx_verify_in {
   const void* target;
   const float* q;

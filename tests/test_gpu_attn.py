@@ -220,3 +220,64 @@ def test_captured_step_replays_with_other_lengths():
 def test_one_row_over_many_ranges(D, Hq, Hkv, L):
     s = kv.Step([1], [L], Hq=Hq, Hkv=Hkv, D=D, page=64, seed=D)
     kv.check_attn(s, *s.run())
+
+
+@pytest.mark.parametrize("B,prefix,cu", [(300, 0, True), (300, 40, True), (257, 0, False), (65, 0, False)])
+def test_many_sequences(B, prefix, cu):
+    rows = [2] * B if not cu else [1 + b % 3 if b % 7 else 0 for b in range(B)]
+    s = kv.Step(rows, [rows[b] + (53 * b) % 700 for b in range(B)], prefix=prefix, Hq=4, Hkv=2, D=64, page=32, seed=B, cu=cu)
+    kv.check_attn(s, *s.run())
+
+
+def test_a_prefix_too_long_for_the_wider_form():
+    s = kv.Step([1] * 7, [40 + 90 * b for b in range(7)], prefix=32800, Hq=8, Hkv=1, D=64, page=128, fmt="e4m3", seed=21)
+    kv.check_attn(s, *s.run())
+
+
+def _bound(s):
+    n = s.Hq * s.D
+    t = dict(q=s.q.reshape(s.R, n).cuda(), out=torch.zeros(s.R, n, dtype=torch.bfloat16, device="cuda"), lse=torch.zeros(s.R, s.Hq, device="cuda"))
+    return t, lambda ws, stream=None: lib.attn(s.cache, s.batch, t["q"], n, s.Hq, s.D ** -0.5, t["out"], n, ws, lse=t["lse"], stream=stream)
+
+
+def test_graphs_of_different_batches_share_a_workspace():
+    steps = [kv.Step([2, 1, 3], [700, 90, 1300], prefix=500, Hq=16, Hkv=2, seed=31), kv.Step([1] * 5, [900, 20, 3000, 7, 600], Hq=8, Hkv=2, seed=32),
+             kv.Step([9], [2000], prefix=300, Hq=16, Hkv=2, seed=33)]
+    ws = torch.zeros(max(lib.attn_ws_bytes(s.cache, s.batch, s.Hq) for s in steps), dtype=torch.uint8, device="cuda")
+    calls, want, graphs = [_bound(s) for s in steps], [], []
+    for s, (t, call) in zip(steps, calls):
+        call(ws)
+        torch.cuda.synchronize()
+        kv.check_attn(s, t["out"].cpu(), t["lse"].cpu())
+        want.append((t["out"].clone(), t["lse"].clone()))
+    for t, call in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(ws)
+        graphs.append(g)
+    for i in (0, 1, 2, 1, 0, 2, 2, 0):
+        calls[i][0]["out"].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(calls[i][0]["out"], want[i][0]) and torch.equal(calls[i][0]["lse"], want[i][1]), i
+        torch.randn(1 << 16, device="cuda").sum().item()
+
+
+def test_two_calls_at_once_on_streams_of_their_own():
+    steps = [kv.Step([2, 1, 3], [700, 90, 1300], prefix=500, Hq=16, Hkv=2, seed=31), kv.Step([1] * 5, [900, 20, 3000, 7, 600], Hq=8, Hkv=2, seed=32)]
+    calls = [_bound(s) for s in steps]
+    wss = [torch.zeros(lib.attn_ws_bytes(s.cache, s.batch, s.Hq), dtype=torch.uint8, device="cuda") for s in steps]
+    want = []
+    for (t, call), ws in zip(calls, wss):
+        call(ws)
+        torch.cuda.synchronize()
+        want.append(t["out"].clone())
+        t["out"].zero_()
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (t, call), ws, st in zip(calls, wss, streams):
+            call(ws, stream=st)
+    torch.cuda.synchronize()
+    for (t, _), w in zip(calls, want):
+        assert torch.equal(t["out"], w)

@@ -228,3 +228,32 @@ def test_no_rows_at_all():
         assert lib.lib().dsgx_spec_verify(C.byref(a), ids.data_ptr(), accepted.data_ptr(), ws.data_ptr(), None) == abi.OK
         torch.cuda.synchronize()
         assert accepted.tolist() == [0, 0, 0] and ids.tolist() == [0] * 4
+
+
+def test_graphs_of_different_sizes_share_a_workspace():
+    ds = [_inputs([3] * 40, 70001, "f32", 91, False, [0.8] * 40), _inputs([2, 5], 900, "bf16", 92, True), _inputs([1, 4, 2], 20000, "prob", 93)]
+    sizes = [(len(d["rows"]), sum(d["rows"]), d["target"].shape[1]) for d in ds]
+    ws = torch.zeros(max(lib.spec_verify_ws_bytes(*n) for n in sizes), dtype=torch.uint8, device="cuda")
+    up = lambda t: None if t is None else t.cuda()  # noqa: E731
+    calls, outs, graphs = [], [], []
+    for d, (B, R, V) in zip(ds, sizes):
+        g = {k: up(d[k]) for k in ("target", "draft", "u", "us", "q", "temp")}
+        cu = torch.tensor(np.concatenate([[0], np.cumsum(d["rows"])]), dtype=torch.int32).cuda()
+        tokens, accepted = torch.zeros(R, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+        outs.append((tokens, accepted))
+        calls.append(lambda g=g, V=V, o=outs[-1], cu=cu, d=d: lib.spec_verify(g["target"], V, g["draft"], g["u"], g["us"], *o, ws, max(d["rows"]), cu_rows=cu, q=g["q"], temp=g["temp"],
+                                                                             probs=d["probs"]))
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+    for i in (0, 1, 2, 2, 1, 0, 0):
+        outs[i][0].fill_(77), outs[i][1].fill_(77)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        want = _want(ds[i])
+        assert np.array_equal(outs[i][0].cpu().numpy(), want[0]) and np.array_equal(outs[i][1].cpu().numpy(), want[1]), i
+        torch.randn(1 << 16, device="cuda").sum().item()

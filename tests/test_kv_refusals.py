@@ -99,3 +99,29 @@ def test_packed_arguments_are_the_structs():
     assert lib._APPEND(*a) == bytes(abi.KvAppendIn(*a))
     a = (1, 2, 3, 4, 5, 6, 7, 8, 1 << 40, 2, -11, 12, 13, 14)
     assert lib._VERIFY(*a) == bytes(abi.VerifyIn(*a))
+
+
+def test_types_of_tensors():
+    c, b = _cache(), _batch()
+    t = lambda *n, d=torch.float32: torch.zeros(*n, dtype=d)  # noqa: E731
+    for kw in (dict(rope=t(4, 16, d=torch.bfloat16), rot=16), dict(pos=t(4, d=torch.int64))):
+        with pytest.raises(lib.DsgxError):
+            lib.kv_append(c, b, t(64), 256, t(64), 256, **kw)
+    i32 = torch.int32
+    ok = dict(draft=t(3, d=i32), u=t(3), us=t(1), tokens=t(3, d=i32), accepted=t(1, d=i32), temp=None, cu_rows=None)
+    for bad in (dict(draft=t(3, d=torch.int64)), dict(u=t(3, d=torch.float64)), dict(us=t(1, d=torch.bfloat16)), dict(tokens=t(3, d=torch.int64)), dict(accepted=t(1, d=torch.int16)),
+                dict(temp=t(1, d=torch.float16)), dict(cu_rows=t(2, d=torch.int64))):
+        a = {**ok, **bad}
+        with pytest.raises(lib.DsgxError):
+            lib.spec_verify(t(3, 50), 50, a["draft"], a["u"], a["us"], a["tokens"], a["accepted"], t(8), 3, cu_rows=a["cu_rows"], temp=a["temp"])
+
+
+@pytest.mark.parametrize("D,fmt,Hkv,G", [(64, abi.FMT_BF16, 5, 3), (128, abi.FMT_BF16, 8, 8), (128, abi.FMT_BF16, 1, 1), (256, abi.FMT_BF16, 1, 64)])
+def test_the_largest_batch_sizes_the_workspace(D, fmt, Hkv, G):
+    c = _cache(Hkv=Hkv, D=D, head_stride=D, tok_stride=Hkv * D, page_stride=16 * Hkv * D)
+    need = lambda **kw: lib.attn_ws_bytes(c, _batch(**kw), Hkv * G)  # noqa: E731
+    whole = need(B=40, rows=200, max_rows=8, max_len=100)
+    assert whole == need(B=40, rows=200, max_rows=200, max_len=90000, prefix_len=50000, prefix=0x400, table_ld=9000)
+    for B in (1, 7, 40):
+        for rows in (B, 2 * B, 200):
+            assert 0 < need(B=B, rows=rows, max_rows=rows) <= whole
