@@ -307,6 +307,9 @@ def kv_batch(rows, max_rows, max_len, lens, table, cu_rows=None, prefix_len=0, p
     for t in (lens, table, cu_rows, prefix):
         if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous()):
             raise DsgxError(abi.EINVAL, "kv_batch: lens, table, cu_rows and prefix are contiguous 32-bit integers")
+    B = table.shape[0]
+    if table.dim() != 2 or lens.numel() < B or (cu_rows is not None and cu_rows.numel() < B + 1):
+        raise DsgxError(abi.EINVAL, "kv_batch: %d lengths and %s bounds for the table %s" % (lens.numel(), None if cu_rows is None else cu_rows.numel(), tuple(table.shape)))
     return abi.KvBatch(_ptr(cu_rows), _ptr(lens), _ptr(table), _ptr(prefix), table.shape[0], rows, max_rows, max_len, table.shape[1], prefix_len)
 
 
@@ -355,8 +358,11 @@ def spec_verify(target, V, draft, u, us, tokens, accepted, ws, max_rows, cu_rows
     if tokens.dtype is not _I32 or accepted.dtype is not _I32 or us.dtype is not _F32 or any(t is not None and t.dtype is not _I32 for t in (draft, cu_rows)) or \
             any(t is not None and t.dtype is not _F32 for t in (u, temp)):
         raise DsgxError(abi.EINVAL, "spec_verify: ids and bounds are i32, random numbers and temperatures f32")
+    B, rows = accepted.numel(), tokens.numel()
+    if us.numel() < B or (cu_rows is not None and cu_rows.numel() < B + 1) or (temp is not None and temp.numel() < B) or any(t is not None and t.numel() < rows for t in (draft, u)):
+        raise DsgxError(abi.EINVAL, "spec_verify: ids, bounds or random numbers missing for %d sequences of %d rows" % (B, rows))
     a = _VERIFY(target.data_ptr(), 0 if q is None else q.data_ptr(), 0 if draft is None else draft.data_ptr(), 0 if cu_rows is None else cu_rows.data_ptr(),
-                0 if u is None else u.data_ptr(), us.data_ptr(), 0 if temp is None else temp.data_ptr(), ldt or V, ldq or V, kind, V, accepted.numel(), tokens.numel(), max_rows)
+                0 if u is None else u.data_ptr(), us.data_ptr(), 0 if temp is None else temp.data_ptr(), ldt or V, ldq or V, kind, V, B, rows, max_rows)
     rc = L.dsgx_spec_verify(a, tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), _stream(stream))
     if rc:
         _check(rc)

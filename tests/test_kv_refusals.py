@@ -110,10 +110,19 @@ def test_types_of_tensors():
     i32 = torch.int32
     ok = dict(draft=t(3, d=i32), u=t(3), us=t(1), tokens=t(3, d=i32), accepted=t(1, d=i32), temp=None, cu_rows=None)
     for bad in (dict(draft=t(3, d=torch.int64)), dict(u=t(3, d=torch.float64)), dict(us=t(1, d=torch.bfloat16)), dict(tokens=t(3, d=torch.int64)), dict(accepted=t(1, d=torch.int16)),
-                dict(temp=t(1, d=torch.float16)), dict(cu_rows=t(2, d=torch.int64))):
+                dict(temp=t(1, d=torch.float16)), dict(cu_rows=t(2, d=torch.int64)), dict(us=t(0)), dict(draft=t(2, d=i32)), dict(u=t(1)), dict(cu_rows=t(1, d=i32)), dict(temp=t(0))):
         a = {**ok, **bad}
         with pytest.raises(lib.DsgxError):
             lib.spec_verify(t(3, 50), 50, a["draft"], a["u"], a["us"], a["tokens"], a["accepted"], t(8), 3, cu_rows=a["cu_rows"], temp=a["temp"])
+
+
+def test_batches_that_miss_lengths():
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
+    lib.kv_batch(4, 2, 16, i(2), i(2, 3), cu_rows=i(3))
+    for kw in (dict(lens=i(1)), dict(cu_rows=i(2)), dict(table=i(6))):
+        a = dict(dict(lens=i(2), table=i(2, 3), cu_rows=i(3)), **kw)
+        with pytest.raises(lib.DsgxError):
+            lib.kv_batch(4, 2, 16, a["lens"], a["table"], cu_rows=a["cu_rows"])
 
 
 @pytest.mark.parametrize("D,fmt,Hkv,G", [(64, abi.FMT_BF16, 5, 3), (128, abi.FMT_BF16, 8, 8), (128, abi.FMT_BF16, 1, 1), (256, abi.FMT_BF16, 1, 64)])
