@@ -1,6 +1,7 @@
 // Verification of drafted tokens against the target's distribution from given random numbers (include/dsgx.h). The result is whole
 // numbers that lie next to borders (a cumulative sum over the vocabulary against a random threshold), so all sums and probabilities are
-// f64: with f32 exponentials about one draw in a hundred of a flat distribution over 10^5 tokens would come out one token off.
+// f64: with f32 exponentials about one draw in a hundred of a flat distribution over 10^5 tokens would come out one token off. (One sum that no
+// draw depends on is the exception, see k_stats.)
 //
 // Two launches: k_stats reads every row of logits once and leaves, for each piece of it, the maximum, the sum of exp and the lowest
 // id of the maximum, and for the row what its draft's target and drafter are; k_weights judges its sequence's drafts (every workgroup for
@@ -9,8 +10,7 @@
 //
 // A piece is as many chunks of 4096 ids as let the whole launch be on the card at once (pieces_of): the chain from a workgroup's first load to
 // its last takes about 7 us in k_weights, and a second round of workgroups would wait for it again.
-// Measured, both launches: 16 x 5 rows of 131072 f32 logits 27.8 us (13.3 + 14.5, 42 + 8.4 + 8.4 MB), 224 rows of 100003 in bf16 40.5 (22.2 of
-// them exponentials), 32 x 4 of 65537 probabilities 12.4, 2 rows of 32768 14.0.
+// Measured, both launches: 16 x 5 rows of 131072 f32 logits 27.8 us (13.3 + 14.5, 42 + 8.4 + 8.4 MB), 224 rows of 100003 in bf16 31.9 (13.7 + 18.2), 32 x 4 of 65537 probabilities 12.4, 2 rows of 32768 14.0.
 #include "abi_internal.h"
 #include "common.cuh"
 
@@ -133,7 +133,7 @@ __constant__ double kExp2[kTable] = {
 };
 struct Exp {
   double itl, max;    // kTable / (T ln 2)
-  float lo;           // max - 700 T
+  float lo, rough;    // max - 700 T; 1 / (T ln 2)
   const double* tab;  // kExp2 in LDS
 };
 // lo is rounded to max's bits: no further from it than the exponent reaches, and below it. Where 700 T is less than half a step of max, what
@@ -143,7 +143,8 @@ __device__ __forceinline__ Exp exp_of(float max, float T, double it, const doubl
   const float up = __uint_as_float(__float_as_uint(lo) + (lo > 0.f ? 1u : -1u)), below = __uint_as_float(max > 0.f ? __float_as_uint(max) - 1u : __float_as_uint(max) + 1u);
   if (((double)max - (double)lo) * it > 705.0) lo = up;
   if (lo == max && max != __builtin_inff()) lo = below, it = 700.0 / ((double)max - (double)lo);
-  return Exp{it * (kTable * 1.4426950408889634074), (double)max, lo, tab};
+  const double l2 = it * 1.4426950408889634074;
+  return Exp{l2 * kTable, (double)max, lo, l2 > 3e38 ? 3e38f : (float)l2, tab};
 }
 template <bool ZERO>
 __device__ __forceinline__ double exp_at(const Exp& e, float x) {
@@ -265,7 +266,12 @@ __device__ __forceinline__ void loads_stay() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int KIND>
+// FINE: the row's probabilities are compared with a drafter's id by id, and an error of the sum moves the borders of a draw: f64. Else the sum
+// stands behind the draft's own probability alone (a draw from p itself does not need it), and exponentials in f32 do, added in f32 by
+// sixteens. A term 2^-z of the largest is off by z 2^-23 (difference, scaling) and 2^-23 (the exponential), sixteen of them by 2^-22, all of
+// random sign: with the sum's bulk at z <= 6, 10^-6 if every sign were the same. That decides otherwise than f64 for one draft in a million
+// at most: 224 bf16 rows of 100003 take 13.7 us instead of 22.2.
+template <int KIND, bool FINE>
 __global__ void __launch_bounds__(kStatThreads) k_stats(VerifyArgs a) {
   constexpr int U = kUnit<KIND>, NU = kStatPer / U;
   const dsgx_verify_in& in = a.in;
@@ -320,7 +326,14 @@ __global__ void __launch_bounds__(kStatThreads) k_stats(VerifyArgs a) {
 #pragma unroll
         for (int i = U - 1; i >= 0; --i) arg = x[k][i] == m ? c * kStatChunk + (k * kStatThreads + (int)threadIdx.x) * U + i : arg;
     }
-    if (!greedy && m != -__builtin_inff()) {
+    if (!greedy && m != -__builtin_inff() && !FINE) {
+      float f = 0.f;
+#pragma unroll
+      for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < U; ++i) f += __builtin_amdgcn_exp2f((x[k][i] - m) * e.rough);
+      s += (double)f;
+    } else if (!greedy && m != -__builtin_inff()) {
 #pragma unroll
       for (int k = 0; k < NU; ++k)
 #pragma unroll
@@ -590,8 +603,9 @@ __global__ void __launch_bounds__(kThreads) k_weights(VerifyArgs a) {
 
 template <int KIND>
 int launch(const VerifyArgs& a, hipStream_t st) {
-  if (KIND != 2 && a.in.rows) {
-    hipLaunchKernelGGL(k_stats<KIND>, dim3(a.ns, a.in.rows), dim3(kStatThreads), 0, st, a);
+  if constexpr (KIND != 2) if (a.in.rows) {
+    if (a.in.q) hipLaunchKernelGGL((k_stats<KIND, true>), dim3(a.ns, a.in.rows), dim3(kStatThreads), 0, st, a);
+    else hipLaunchKernelGGL((k_stats<KIND, false>), dim3(a.ns, a.in.rows), dim3(kStatThreads), 0, st, a);
     DSGX_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL(k_weights<KIND>, dim3((a.nc + a.sw - 1) / a.sw, a.in.B), dim3(kThreads), 0, st, a);
@@ -604,7 +618,7 @@ constexpr size_t kCountBytes = 65536 * sizeof(int);  // first in the workspace w
 size_t stat_bytes(int rows, int nc) { return align256((size_t)rows * nc * sizeof(Stat)) + align256((size_t)rows * sizeof(Draft)); }
 size_t sums_bytes(int B, int nc) { return align256((size_t)B * nc * sizeof(Sums)); }
 // Chunks a piece, so that `rows` rows of nc chunks are about `room` workgroups (or pieces are `most` long).
-// k_stats, 224 bf16 rows of 25 chunks: 23.5 to 24.4 us from one to five chunks a piece; 80 f32 rows of 32: 15.0 us in 2560 workgroups,
+// k_stats (in f64), 224 bf16 rows of 25 chunks: 23.5 to 24.4 us from one to five chunks a piece; 80 f32 rows of 32: 15.0 us in 2560 workgroups,
 // 14.0 in 1280. k_weights, 16 sequences of 32 chunks: 17.0 us in 512 workgroups, 14.5 in 256; 48 of 25: 24.4 in 1200, 21.8 in 624,
 // 19.6 in 432, 18.3 in 240.
 int pieces_of(int rows, int nc, int room, int most) {

@@ -388,7 +388,8 @@ DSGX_API size_t dsgx_attn_ws_bytes(const dsgx_kv_cache* cache, const dsgx_kv_bat
 DSGX_API int dsgx_attn(const dsgx_kv_cache* cache, const dsgx_kv_batch* batch, const uint16_t* q, int64_t ldq, int Hq, float scale,
                        uint16_t* out, int64_t ldo, float* lse, void* ws, void* stream);
 
-/* Verification of drafted tokens by rejection sampling from given random numbers, all in f64. Sequence b has the rows
+/* Verification of drafted tokens by rejection sampling from given random numbers, in f64 (p(draft) of logits without a drafter's
+   probabilities: to 10^-6 of itself). Sequence b has the rows
    cu_rows[b] .. cu_rows[b + 1] - 1 of the target (null: max_rows rows each), one more than it has drafts: row i judges draft i, the last
    row follows them all. Row r: the target p_r = softmax(target[r] / temp[b]) (temp <= 0: all on the largest logit, the lowest id of
    equals), or with probs target[r] itself; draft[r], u[r] in [0, 1) and the drafter's probabilities q[r] (null: the

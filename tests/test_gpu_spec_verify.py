@@ -207,16 +207,30 @@ def test_a_nan_or_infinity_in_any_chunk_refuses_the_row(where):
 @pytest.mark.parametrize("T", [1e-3, 1e-6, 3e-9, 1e-10, 1e-30, 1e-44])
 def test_temperatures_near_zero(T):
     """down to where 700 T is less than a step of the maximum; then only the largest logits' ids are left, evenly"""
-    d = _inputs([3, 2, 4], 6000, "f32", 79, False, [T] * 3)
-    d["target"][2, [7, 4500]] = 30.0
-    _check(d)
+    for sharp in (False, True):
+        d = _inputs([3, 2, 4], 6000, "f32", 79, sharp, [T] * 3)
+        d["target"][2, [7, 4500]] = 30.0
+        _check(d)
 
 
 @pytest.mark.parametrize("T", [1e6, 1e30, 3e38])
 def test_temperatures_that_flatten_everything(T):
-    d = _inputs([3, 2, 4], 6000, "f32", 80, False, [T] * 3)
-    d["target"][:, 100:4500] = -float("inf")
-    _check(d)
+    for sharp in (False, True):
+        d = _inputs([3, 2, 4], 6000, "f32", 80, sharp, [T] * 3)
+        d["target"][:, 100:4500] = -float("inf")
+        _check(d)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_the_drafts_border_without_probabilities(kind):
+    """u on either side of p(draft), 4 * 10^-6 of it away: the border moves by 10^-6 at most, u is rounded to 2^-24"""
+    d = _inputs([2] * 60, 30011, kind, 95, True, [0.4 + 0.05 * b for b in range(60)])
+    p = torch.softmax(d["target"].double() / d["temp"].double().repeat_interleave(2)[:, None], -1)
+    at = p.gather(1, d["draft"].long()[:, None])[:, 0]
+    side = torch.where(torch.arange(120) // 2 % 2 == 0, 1 - 4e-6, 1 + 4e-6)
+    d["u"] = (at * side).float()
+    tokens, accepted = _check(d)
+    assert accepted.tolist() == [1, 0] * 30
 
 
 def test_no_rows_at_all():
