@@ -1027,9 +1027,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_both(AttnArgs a) {
 
 // The ranges' outputs of a row's head joined by their maxima: WPH waves a head, D / 4 lanes a range
 template <int D, int WPH>
-__global__ void __launch_bounds__(WPH == 16 ? 1024 : 256) k_combine(AttnArgs a) {
+__global__ void __launch_bounds__(WPH > 4 ? 64 * WPH : 256) k_combine(AttnArgs a) {
   constexpr int LR = D / 4, RW = kWave / LR, STEP = RW * WPH;  // lanes a range, ranges a wave, ranges a turn
-  constexpr int WAVES = WPH == 16 ? 16 : 4;
+  constexpr int WAVES = WPH > 4 ? WPH : 4;
   __shared__ v4f_t racc[WAVES][LR];
   __shared__ float rl[WAVES], rm[WAVES];
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), part = wave % WPH, r = blockIdx.x, head = (int)blockIdx.y * (WAVES / WPH) + wave / WPH;
@@ -1231,10 +1231,10 @@ int launch(AttnArgs& a, const Layout& y, hipStream_t st) {
     if (int rc = launch_part<D, F8>(a, y.ko, own, kOwnOnly, st)) return rc;
   }
   if (!a.pre.splits && !a.own.target) return DSGX_OK;
-  // Waves a head, by how many heads there are and about how many ranges each has: 128 ranges of 32 heads of 256 values 14.5 us by four, 7.5 by
-  // sixteen; 16 of 256 heads 4.8, 5.9; 320 heads 9.8, 13.9.
+  // Waves a head, by how many heads there are and about how many ranges each has: 128 ranges of 32 heads of 256 values 14.5 us by four waves, 7.4
+  // by eight, 7.6 by sixteen; 102 of 320 heads 9.8, 9.5, 13.9; 16 of 256 heads 4.8 by four, 5.9 by sixteen.
   const int64_t ranges = a.pre.splits + std::min<int64_t>(a.b.max_len / a.own.least, (int64_t)a.own.target * a.own.heads / ((int64_t)a.c.Hkv * a.b.B));
-  if ((int64_t)a.b.rows * a.Hq <= 256 && ranges > 32) hipLaunchKernelGGL((k_combine<D, 16>), dim3(a.b.rows, a.Hq), dim3(1024), 0, st, a);
+  if ((int64_t)a.b.rows * a.Hq <= 512 && ranges > 32) hipLaunchKernelGGL((k_combine<D, 8>), dim3(a.b.rows, a.Hq), dim3(512), 0, st, a);
   else if ((int64_t)a.b.rows * a.Hq <= 1024) hipLaunchKernelGGL((k_combine<D, 4>), dim3(a.b.rows, a.Hq), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_combine<D, 1>), dim3(a.b.rows, (a.Hq + 3) / 4), dim3(256), 0, st, a);
   DSGX_HIP(hipGetLastError());
