@@ -44,7 +44,7 @@ struct AttnArgs {
   uint16_t* out;
   float *lse, *part;  // part: [places][cols][D], the prefix's first
   float2* ml;         // [places][cols]
-  int pre_blocks;     // of a launch for both
+  int pre_blocks;     // workgroups for the prefix, a multiple of 8
   int32_t* plan;      // [4 + B]: tokens a range, heads a workgroup; from 4 on every sequence's first item
   int64_t ldq, ldo;
   int Hq, G, page_shift;
@@ -218,9 +218,10 @@ __device__ __forceinline__ Item uniform(const Item& t) {
               uni((int)t.alone) != 0};
 }
 __device__ __forceinline__ Item prefix_item(const AttnArgs& a, int i, bool& any) {
-  // The tiles that read the same tokens run on the same XCD (workgroup i runs on XCD i % 8) next to each other, out of its L2
-  const int pair = i / 8 / a.pre.tiles * 8 + i % 8, groups = a.c.Hkv / a.pre.heads, split = pair / groups;
-  Item t{(table_t)(uintptr_t)a.b.prefix, pair % groups * a.pre.heads, 0, a.b.rows, a.b.prefix_len, split * a.pre.chunk, 0, i / 8 % a.pre.tiles, 0, 0, false, false};
+  // The tiles that read the same tokens run on the same XCD (workgroup i runs on XCD i % 8) next to each other, out of its L2: an eighth of all
+  // for every XCD, in order. (Whole ranges for an XCD, 20001 tokens in 3 for 4 heads of 256 and 38 tiles took 582 us instead of 437.)
+  const int n = i % 8 * (a.pre_blocks / 8) + i / 8, groups = a.c.Hkv / a.pre.heads, pair = n / a.pre.tiles, split = pair / groups;
+  Item t{(table_t)(uintptr_t)a.b.prefix, pair % groups * a.pre.heads, 0, a.b.rows, a.b.prefix_len, split * a.pre.chunk, 0, n % a.pre.tiles, 0, 0, false, false};
   t.hi = min(t.len, t.lo + a.pre.chunk), t.next = (int64_t)a.pre.tiles * a.pre.cols;
   t.place = (int64_t)(split * a.c.Hkv + t.head) * t.next + (int64_t)t.tile * a.pre.cols;
   any = split < a.pre.splits;
@@ -1112,7 +1113,8 @@ int round_up(int64_t v, int m) { return (int)((v + m - 1) / m * m); }
 // How `cols` query columns over the same tokens are worked on: 16 or 32 a workgroup from registers, 64 or 128 over tiles in LDS.
 // 128 against 64, D 128: 6 x 8 rows of 16 heads over each of 4, 5000 to 8000 tokens 33.5 us, 37.2; 8011 tokens before 48 rows of 64 heads over 8 28.8, 36.2.
 // D 256 by 128 columns takes over half a SIMD's registers, and its one wave a SIMD waits for whatever it waits for: 5 rows of 64 heads over one, 50001
-// tokens 53.2 us (e4m3 51.9), by 64 columns 50.1 (43.0); 20000 before 300 rows of 32 heads 688 (680), 566 (539). By 16 from registers it is so
+// tokens 53.2 us (e4m3 51.9), by 64 columns 50.1
+// (43.0; both before tiles over the same tokens shared an XCD). By 16 from registers it is so
 // too for BF16: 16 rows of 8 heads over each of 2, 300 to 8000 tokens 28.7 us, by 64 columns 23.5 (e4m3 18.0, 22.8); and behind a prefix one launch
 // has both.
 enum Kind { kNarrow16, kNarrow32, kWide64, kWide128 };
@@ -1162,6 +1164,7 @@ Layout make_layout(const dsgx_kv_cache& c, const dsgx_kv_batch& b, int Hq) {
     const int64_t each = (int64_t)(c.Hkv / y.pre.heads) * y.pre.tiles;
     y.both = y.kp == y.ko || (y.kp == kWide128 && y.ko <= kNarrow32);
     double pre_room = cus * resident(y.kp, c.D);
+    // (8011 tokens before 48 rows: at least half of it for the prefix 36.1 us, two thirds 35.4, four fifths 39.5.)
     // In one launch the room is shared by the work (tokens times tiles; of max_len half, on average), two thirds at least for the prefix, whose
     // ranges are cut here; what is left of it is the own tokens', or all of it where they are most of the work and come second.
     const double mine = 0.5 * b.B * b.max_len * (((int64_t)b.max_rows * G + y.own.cols - 1) / y.own.cols), theirs = (double)b.prefix_len * y.pre.tiles;
@@ -1217,7 +1220,7 @@ int launch(AttnArgs& a, const Layout& y, hipStream_t st) {
   const unsigned own = ((unsigned)y.own_grid + 7) / 8 * 8;  // (more than there are items do nothing)
   if (a.pre.splits) {
     const int64_t pairs = (int64_t)a.pre.splits * (a.c.Hkv / a.pre.heads);
-    const unsigned pre = (unsigned)((pairs + 7) / 8 * 8 * a.pre.tiles);
+    const unsigned pre = (unsigned)((pairs * a.pre.tiles + 7) / 8 * 8);
     a.pre_blocks = (int)pre;
     if (y.kp == y.ko) {
       if (int rc = launch_part<D, F8>(a, y.kp, pre + own, kBoth, st)) return rc;
