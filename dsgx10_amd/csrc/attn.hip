@@ -8,8 +8,8 @@
 // Bound by the cache's bytes for few columns, by the matrix unit (and, with e4m3, the staging beside it) for many, and below about 20 us by the
 // chain of a launch: bounds and lengths, page numbers, keys, the waves' join. Whole calls (a large read reaches 7.1 TB/s, a large product 1.4 to
 // 1.6 PFLOP/s): 69 rows of 32 heads over 32 ragged e4m3 sequences, 178 MB, 51 us (44 + 8; 3.5 TB/s); 5 rows of 64 heads of 256 over one, 50001
-// tokens, 60 us (50 + 10; 0.27 PFLOP/s); 8011 tokens before 48 rows of 64 heads with 37 to 600 of their own, 40 us (34 + 7); 32768 before 300 rows of
-// 32 heads, e4m3, 215 us (0.76 PFLOP/s); one row over 301 tokens 10 us.
+// tokens, 51 us (45 + 9.5; 0.32 PFLOP/s); 8011 tokens before 48 rows of 64 heads with 37 to 600 of their own, 40 us (34 + 7); 32768 before 300 rows of
+// 32 heads, e4m3, 209 us (0.78 PFLOP/s); one row over 301 tokens 10 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1112,11 +1112,10 @@ int round_up(int64_t v, int m) { return (int)((v + m - 1) / m * m); }
 
 // How `cols` query columns over the same tokens are worked on: 16 or 32 a workgroup from registers, 64 or 128 over tiles in LDS.
 // 128 against 64, D 128: 6 x 8 rows of 16 heads over each of 4, 5000 to 8000 tokens 33.5 us, 37.2; 8011 tokens before 48 rows of 64 heads over 8 28.8, 36.2.
-// D 256 by 128 columns takes over half a SIMD's registers, and its one wave a SIMD waits for whatever it waits for: 5 rows of 64 heads over one, 50001
-// tokens 53.2 us (e4m3 51.9), by 64 columns 50.1
-// (43.0; both before tiles over the same tokens shared an XCD). By 16 from registers it is so
-// too for BF16: 16 rows of 8 heads over each of 2, 300 to 8000 tokens 28.7 us, by 64 columns 23.5 (e4m3 18.0, 22.8); and behind a prefix one launch
-// has both.
+// D 256 by 128 columns takes over half a SIMD's registers, and its one wave a SIMD waits for whatever it waits for: 5 rows of 64 heads over
+// one, 50001 tokens 53.2 us (e4m3 51.9), by 64 columns 50.1 (43.0; both before tiles over the same tokens shared an XCD). By 16 from registers it
+// is so too for BF16: 16 rows of 8 heads over each of 2, 300 to 8000 tokens 28.7 us, by 64 columns 23.5 (e4m3 18.0, 22.8); and behind a prefix
+// one launch has both.
 enum Kind { kNarrow16, kNarrow32, kWide64, kWide128 };
 Kind kind_of(int64_t cols, int D, bool f8, bool prefix) {
   if (D == 256) return cols <= 16 && f8 && !prefix ? kNarrow16 : kWide64;
