@@ -8,7 +8,7 @@
 // Bound by the cache's bytes for few columns, by the matrix unit (and, with e4m3, the staging beside it) for many, and below about 20 us by the
 // chain of a launch: bounds and lengths, page numbers, keys, the waves' join. Whole calls (a large read reaches 7.1 TB/s, a large product 1.4 to
 // 1.6 PFLOP/s): 69 rows of 32 heads over 32 ragged e4m3 sequences, 178 MB, 51 us (44 + 8; 3.5 TB/s); 5 rows of 64 heads of 256 over one, 50001
-// tokens, 51 us (45 + 9.5; 0.32 PFLOP/s); 8011 tokens before 48 rows of 64 heads with 37 to 600 of their own, 40 us (34 + 7); 32768 before 300 rows of
+// tokens, 49 us (44.5 + 9.5 alone; 0.33 PFLOP/s); 8011 tokens before 48 rows of 64 heads with 37 to 600 of their own, 40 us (34 + 7); 32768 before 300 rows of
 // 32 heads, e4m3, 209 us (0.78 PFLOP/s); one row over 301 tokens 10 us.
 #include <algorithm>
 #include <cmath>
